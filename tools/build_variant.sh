@@ -8,7 +8,7 @@ cd "$(dirname "$0")/../diffalign_amd"
 NAME=$1; FILE=$2; shift; shift
 BASE=${FILE%.hip}
 mkdir -p csrc/_var
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Icsrc "$@" -c ${SRC:-csrc/$FILE} -o csrc/_var/${BASE}_$NAME.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -Icsrc "$@" -c ${SRC:-csrc/$FILE} -o csrc/_var/${BASE}_$NAME.o
 OBJS=$(ls csrc/_obj/*.o | grep -v "/$BASE.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o libdiffalign_hip_$NAME.so $OBJS csrc/_var/${BASE}_$NAME.o
 echo built libdiffalign_hip_$NAME.so
