@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get('DA_LIB') or os.path.join(_HERE, 'libdiffalign_hip.so'
 _lib: Optional[C.CDLL] = None
 
 c_f = C.c_void_p  # all device pointers travel as void*
-ABI_VERSION = 3      # DA_ABI_VERSION of include/diffalign_hip.h this binding was written against
+ABI_VERSION = 4      # DA_ABI_VERSION of include/diffalign_hip.h this binding was written against
 
 # Signatures of include/diffalign_hip.h, 'return:arguments' with p = pointer (void*), i = int, q = long long, f = float,
 # s = const char*; set on the library once, so that no call site can truncate a size or pass a float as a double
@@ -45,6 +45,8 @@ SIGNATURES = {
     'da_layernorm_bwd': 'i:pppppppqqip',
     'da_res_ln_fwd': 'i:ppipiipppifpppqip', 'da_res_ln_bwd_workspace': 'q:i', 'da_res_ln_bwd': 'i:pppppiipifppipppqqip',
     'da_relu_dropout': 'i:piqpifp', 'da_relu_dropout_bwd': 'i:pppiqfp',
+    'da_mx8_quant': 'i:pippqiip', 'da_mx8_dequant': 'i:pppiqip', 'da_relu_dropout_bwd_mx8': 'i:pppiqfp',
+    'da_linear_wgrad_mx8_workspace': 'q:qii', 'da_linear_wgrad_mx8': 'i:pppipppqqiip',
     'da_pool_stats_fwd': 'i:ppppqiiip', 'da_linear_wgrad_workspace': 'q:qii', 'da_linear_wgrad': 'i:pppppqqiip',
     'da_pool_stats_bwd': 'i:pppppiiip',
     'da_vb_grad': 'i:ppppppppppppppffppiiiip',

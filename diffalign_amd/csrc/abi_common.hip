@@ -13,7 +13,7 @@ void da_set_error(const char* fmt, ...) {
 
 extern "C" {
 const char* da_last_error(void) { return g_err; }
-// 3 (round 3): da_init added, the two-pass output stage (da_edge_out_g / da_edge_out_finish) removed; 2 (round 2, not bumped at the time):
+// 4: da_mx8_*, da_linear_wgrad_mx8, da_relu_dropout_bwd_mx8, da_attn_head_* added; 3: da_init added, the two-pass output stage (da_edge_out_g / da_edge_out_finish) removed; 2:
 // da_y_film / da_y_update* take the y-chain weights k-major ((in, out)), da_edge_layer_stats resets its ticket word itself
-int da_abi_version(void) { return 3; }
+int da_abi_version(void) { return 4; }
 }

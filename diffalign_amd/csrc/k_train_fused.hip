@@ -11,6 +11,7 @@
 // -- dropout masks are random either way; with p = 0 the blocks are exactly the reference's arithmetic.
 // A row of D floats is held by D/4 lanes as one float4 each (16-byte accesses), 256/D rows per wave pass; grid-stride over rows.
 #include "common.h"
+#include "dropout_util.h"
 
 __device__ __forceinline__ unsigned mix32(unsigned x) {
   x ^= x >> 16; x *= 0x7feb352du; x ^= x >> 15; x *= 0x846ca68bu; x ^= x >> 16;
@@ -202,12 +203,6 @@ __global__ void __launch_bounds__(256) k_relu_drop_bwd(const T* __restrict__ h, 
 
 #define RES_LN_MAX_WG 1024
 static bool res_ln_width_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256; }
-static void drop_consts(float p, unsigned* thr, float* scale) {
-  unsigned t = (unsigned)(p * 65536.f + 0.5f);
-  if (t > 65535u) t = 65535u;
-  *thr = t;
-  *scale = 65536.f / (float)(65536u - t);                                 // the exact keep probability of the 16-bit threshold
-}
 static long long res_ln_grid(long long rows, int D) {
   long long g = (rows * D / 256 + 3) / 4;                                  // a wave pass covers 256 floats
   if (g < 1) g = 1;

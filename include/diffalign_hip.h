@@ -17,9 +17,10 @@ extern "C" {
 #endif
 
 /* Version of this header's contracts; a binding built against another version must refuse the library (diffalign_amd/_lib.py does).
- * 3: da_init, the bf16-storage training kernels (da_attn_core_*_bf16, da_linear_wgrad_mixed) and the fused residual blocks (da_res_ln_*, da_relu_dropout*) added, da_edge_out_g / da_edge_out_finish / da_skip_grad removed.  2: da_y_film / da_y_update / da_y_update_film / da_y_pre expect the
+ * 4: 8-bit activation checkpoints (da_mx8_*, da_linear_wgrad_mx8, da_relu_dropout_bwd_mx8) and the per-head attention core (da_attn_head_*)
+ * added.  3: da_init, the bf16-storage training kernels (da_attn_core_*_bf16, da_linear_wgrad_mixed) and the fused residual blocks (da_res_ln_*, da_relu_dropout*) added, da_edge_out_g / da_edge_out_finish / da_skip_grad removed.  2: da_y_film / da_y_update / da_y_update_film / da_y_pre expect the
  * y-chain weights k-major, i.e. transposed to (in, out); da_edge_layer_stats puts its ticket word back to zero itself. */
-#define DA_ABI_VERSION 3
+#define DA_ABI_VERSION 4
 int da_abi_version(void);
 const char* da_last_error(void);
 /* Per-device set-up that must not run under stream capture (today: the device address of da_edge_in_sym_static's scratch).  Call once
@@ -192,6 +193,24 @@ int da_res_ln_bwd(const float* s, const float* gamma, const float* d_out, const 
  * backward: dx = dy / (1 - p) where the stored result is non-zero, else 0 (no mask kept; dx may alias dy). */
 int da_relu_dropout(void* h, int is_bf16, long long numel, const long long* seed, int salt, float p, void* stream);
 int da_relu_dropout_bwd(const void* h, const void* dy, void* dx, int is_bf16, long long numel, float p, void* stream);
+/* ---- 8-bit activation checkpoints of the training step (the reference keeps full-width activations for loss.backward(),
+ * training/helpers.py:139-142).  MXINT8: 32 consecutive channels of a row share the scale 2^(b-127) (one byte b), an element is an int8 q and
+ * stands for q / 64 * 2^(b-127); b is the smallest in [27, 254] at which the group's largest magnitude rounds to 127 or less, 255 (codes 0: the
+ * group stands for NaN) where the group holds an infinity or NaN.  codes (rows, D), scales (rows, ceil(D / 32)). ---- */
+
+/* Quantise x (rows, D) fp32 or bf16 (x_bf16).  keep_nonzero: an element other than zero gets a code other than zero.  Any D >= 1; D % 32
+ * == 0 with x 16-byte and codes 8-byte aligned takes the wide path. */
+int da_mx8_quant(const void* x, int x_bf16, void* codes, uint8_t* scales, long long rows, int D, int keep_nonzero, void* stream);
+/* The values, fp32 or bf16 (out_bf16); both exact. */
+int da_mx8_dequant(const void* codes, const uint8_t* scales, void* out, int out_bf16, long long rows, int D, void* stream);
+/* da_relu_dropout_bwd from the codes (numel int8, quantised with keep_nonzero) of the stored result. */
+int da_relu_dropout_bwd_mx8(const void* codes, const void* dy, void* dx, int is_bf16, long long numel, float p, void* stream);
+/* da_linear_wgrad with X (R, in) held in 8 bits: dW (out,in) = dY^T X, db (out) = column sums of dY (NULL: skipped), fp32.  dY fp32 or bf16
+ * (dy_bf16), every product exact, sums fp32, slices folded in order (deterministic).  in, out in {32, 64, 128, 256} with in * out <= 16384
+ * (others: DA_ERR_UNSUPPORTED, workspace -1); dY, dW, db, workspace 16-byte, codes 8-byte aligned; R >= 1. */
+long long da_linear_wgrad_mx8_workspace(long long R, int in_features, int out_features);
+int da_linear_wgrad_mx8(const void* codes, const uint8_t* scales, const void* dY, int dy_bf16, float* dW, float* db, void* workspace,
+                        long long workspace_bytes, long long R, int in_features, int out_features, void* stream);
 /* LayerNorm backward (eps 1e-5; layers.py:341-359): s (rows,D) = the normalised input, dy the gradient of gamma * xhat + beta ->
  * ds (rows,D), dgamma (D), dbeta (D).  D in {32, 64, 128, 256}; s, dy, ds 16-byte aligned; workspace: 8 * 1024 * D bytes for the
  * per-workgroup partial sums of dgamma / dbeta (folded in workgroup order: deterministic). */
