@@ -8,8 +8,10 @@ import math
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
+from . import mx8
 
 
 def _c(t):
@@ -202,6 +204,91 @@ class AttnCoreBF16(Function):
                                               L.ptr(sm), L.ptr(sl), L.ptr(dZ), L.ptr(dwV), L.ptr(dQ), L.ptr(dK), L.ptr(dV), L.ptr(dE1), L.ptr(dE2),
                                               L.ptr(dye1), L.ptr(dye2), L.ptr(ws), ws.numel(), B, n, dx, L.stream()), 'da_attn_core_bwd_bf16')
         return dQ, dK, dV, dE1, dE2, None, dye1, dye2, None
+
+
+class HeadAttnCore(Function):
+    """The core of NodeEdgeBlockImproved (layers.py:115-141) between the q/k/v/e_mul/e_add projections and e_out / the y_x FiLM; called through
+    head_attention.  `save`: leave the scores and softmax statistics for the backward, and E1 as `checkpoint` says ('none': as it is,
+    'mx8': 8 bits, written by the forward kernel while it reads E1)."""
+
+    @staticmethod
+    def forward(ctx, Q, K, V, E1, E2, nm_u8, groups, n_head, qscale, cap, checkpoint, save):
+        B, n, dx = Q.shape
+        dev = Q.device
+        Y, wV = torch.empty_like(E1), torch.empty_like(Q)
+        S = st = codes = scales = None
+        if save:
+            S, st = torch.empty(B, n, n, n_head, device=dev), torch.empty(B, n, n_head, 2, device=dev)
+            if checkpoint == 'mx8':
+                codes = torch.empty(E1.shape, dtype=torch.int8, device=dev)
+                scales = torch.empty(B, n, n, dx // mx8.GROUP, dtype=torch.uint8, device=dev)
+        with mx8.on_device_of(Q):
+            L.check(L.lib().da_attn_head_fwd(L.ptr(Q), L.ptr(K), L.ptr(V), L.ptr(E1), L.ptr(E2), int(E1.dtype == torch.bfloat16), L.ptr(nm_u8),
+                                             L.ptr(groups), qscale, cap, L.ptr(Y), L.ptr(wV), L.ptr(S), L.ptr(st), L.ptr(codes), L.ptr(scales), B, n, dx,
+                                             n_head, L.stream()), 'da_attn_head_fwd')
+        if save:
+            ctx.save_for_backward(Q, K, V, nm_u8, wV, S, st, *((E1,) if codes is None else (codes, scales)))
+            ctx.meta = (n_head, qscale, cap)
+        return Y, wV
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dY, dwV):
+        Q, K, V, nm_u8, wV, S, st, *e1 = ctx.saved_tensors
+        n_head, qscale, cap = ctx.meta
+        B, n, dx = Q.shape
+        dY, dwV = mx8._aligned(dY), _c16(dwV)
+        E1, codes, scales = (e1[0], None, None) if len(e1) == 1 else (None, *e1)
+        dQ, dK, dV = torch.empty_like(Q), torch.empty_like(Q), torch.empty_like(Q)
+        dE1, dE2 = torch.empty_like(dY), torch.empty_like(dY)
+        with mx8.on_device_of(Q):
+            # the workspace is this call's own: two captured graphs that are replayed side by side must not share one
+            ws = torch.empty(L.lib().da_attn_head_bwd_workspace(B, n, dx, n_head), dtype=torch.uint8, device=Q.device)
+            L.check(L.lib().da_attn_head_bwd(L.ptr(Q), L.ptr(K), L.ptr(V), L.ptr(E1), L.ptr(codes), L.ptr(scales), L.ptr(nm_u8), qscale, cap, L.ptr(wV),
+                                             L.ptr(S), L.ptr(st), L.ptr(dY), int(dY.dtype == torch.bfloat16), L.ptr(dwV), L.ptr(dQ), L.ptr(dK), L.ptr(dV),
+                                             L.ptr(dE1), L.ptr(dE2), L.ptr(ws), ws.numel(), B, n, dx, n_head, L.stream()), 'da_attn_head_bwd')
+        return dQ, dK, dV, dE1, dE2, None, None, None, None, None, None, None
+
+
+def head_attention_built(dx: int, n_head: int) -> bool:
+    """Whether da_attn_head_* has the shape: 4, 8, 16, .. 128 channels per head, dx <= 512 (256 with 4 channels per head)."""
+    return n_head >= 1 and dx % n_head == 0 and dx // n_head in (4, 8, 16, 32, 64, 128) and dx <= (256 if dx // n_head == 4 else 512)
+
+
+def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, groups=None, checkpoint='none'):
+    """Per-head edge attention (NodeEdgeBlockImproved, layers.py:115-141): Q, K, V (B,n,dx), E1 = e_mul(E), E2 = e_add(E) (B,n,n,dx) fp32 or
+    bf16, node_mask (B,n) -> (Y (B,n,n,dx) of E1's type, wV (B,n,dx) fp32), differentiable in the five tensors.
+
+      Y = qscale Q_i K_j (1 + m_i m_j E1) + m_i m_j E2        (qscale: 1 / sqrt(dx / n_head) by default)
+      S = sum of Y over a head's channels, cap tanh(S / cap) with cap > 0;  wV = softmax_j(S) V
+
+    E1 and E2 are not looked at where a node of the pair is masked.  The softmax runs over all keys, as in the reference, or with `groups`
+    (B,n) integers over the keys of the query's own group (a node with a negative group is in none: its wV is 0, and so is the wV of
+    every row without a key).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
+    fp32 arithmetic throughout; sums do not depend on timing."""
+    if Q.dim() != 3 or K.shape != Q.shape or V.shape != Q.shape:
+        raise L.DiffAlignHipError(f'head_attention: Q, K, V (B,n,dx) expected, got {tuple(Q.shape)}, {tuple(K.shape)}, {tuple(V.shape)}')
+    B, n, dx = Q.shape
+    if E1.shape != (B, n, n, dx) or E2.shape != E1.shape or E1.dtype != E2.dtype or E1.dtype not in (torch.float32, torch.bfloat16):
+        raise L.DiffAlignHipError(f'head_attention: E1, E2 {(B, n, n, dx)} of one type, fp32 or bf16, expected, got {E1.dtype} {tuple(E1.shape)}, '
+                                  f'{E2.dtype} {tuple(E2.shape)}')
+    if node_mask.shape != (B, n) or (groups is not None and (groups.shape != (B, n) or groups.is_floating_point() or groups.dtype == torch.bool)):
+        raise L.DiffAlignHipError(f'head_attention: node_mask and groups (integers) of shape {(B, n)} expected')
+    if any(t is not None and t.device != Q.device for t in (K, V, E1, E2, node_mask, groups)):
+        raise L.DiffAlignHipError('head_attention: tensors on different devices')
+    if not head_attention_built(dx, n_head):
+        raise L.DiffAlignHipError(f'head_attention: dx = {dx} with {n_head} heads not built')
+    if checkpoint not in ('none', 'mx8'):
+        raise ValueError(f"head_attention: checkpoint {checkpoint!r}: 'none' or 'mx8'")
+    if checkpoint == 'mx8' and dx % mx8.GROUP:
+        raise L.DiffAlignHipError(f"head_attention: checkpoint='mx8' needs dx % {mx8.GROUP} == 0, dx = {dx}")
+    cap = float(cap)
+    if not 0.0 <= cap < math.inf:
+        raise ValueError(f'head_attention: cap = {cap}')
+    save = torch.is_grad_enabled() and any(t.requires_grad for t in (Q, K, V, E1, E2))
+    return HeadAttnCore.apply(_c16(Q), _c16(K), _c16(V), mx8._aligned(E1), mx8._aligned(E2), L.as_u8(node_mask),
+                              None if groups is None else groups.to(torch.int32).contiguous(), n_head,
+                              qscale_of(dx, n_head) if qscale is None else float(qscale), cap, checkpoint, save)
 
 
 class AddLayerNorm(Function):

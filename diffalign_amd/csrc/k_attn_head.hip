@@ -1,0 +1,553 @@
+// Per-head edge attention, forward and backward: the core of NodeEdgeBlockImproved (neuralnet/layers.py:115-141), where the edge-modulated
+// products of a head are summed into one score and the softmax over the keys is per head (the plain block, k_backward.hip, has one per
+// channel).  Per pair (i,j) and channel c of head h(c), m_ij = m_i m_j:
+//   Y_ijc = s Q_ic K_jc (1 + m_ij E1_ijc) + m_ij E2_ijc            the input of e_out
+//   S_ijh = sum over the head's channels of Y;   S' = cap tanh(S / cap) where cap > 0, else S
+//   P_ijh = softmax over the keys j with group_j == group_i >= 0 (all keys without groups);   wV_ic = sum_j P_ijh V_jc
+// A row without a key gets wV = 0.  With G_ijc = dY_ijc + dS_ijh, dS = P (dP - D) (1 - (S'/cap)^2), dP_ijh = dwV_i . V_j and
+// D_ih = dwV_i . wV_i (sums over the head's channels) the gradients are
+//   dE2 = m G;  dE1 = m G s Q K;  dQ_i = sum_j G s (1 + m E1) K_j;  dK_j = sum_i G s (1 + m E1) Q_i;  dV_j = sum_i P dwV_i.
+// The forward leaves S' (B,n,n,H) and the softmax statistics, 4 H bytes a pair beside 2-4 dx for each of E1 and E2: the backward then
+// needs neither E2 nor the scores' sum again, and E1, the one wide operand left, may be held in 8 bits (mx8_util.h).
+//
+// Bound: HBM.  Forward E1, E2 in, Y out; backward E1, dY in, dE1, dE2 out: 3 and 4 (3.5 with 8 bits of E1 beside bf16) streams of B n n dx
+// elements against about 12 operations per element each way.  So every stream is touched once, in 16-byte accesses, and what repeats stays in
+// registers: a lane holds C channels of one head, LP = dx / C lanes (a power of two) a pair, a wave 64 / LP keys at a time for RW query
+// rows, whose Q (dwV, dQ) never move; K_j and V_j are fetched once for the RW rows.  A head's sum runs over df / C neighbouring lanes
+// (DPP).  E1 and E2 are read through a buffer descriptor whose range ends at the rows in hand: a masked pair, a row past the end and a
+// channel past dx get an offset outside it, so the hardware returns the 0 that the formula wants and moves no data.
+#include "mfma_util.h"
+#include "mx8_util.h"
+#include <initializer_list>
+#include <type_traits>
+
+struct HeadArgs {
+  const float *Q, *K, *V;
+  const void *E1, *E2;                  // E1: TE, or its codes (8-bit backward)
+  const uint8_t* E1s;                   // scale bytes of E1's codes
+  const uint8_t* nm;
+  const int* grp;                       // nullable
+  float qscale, cap;
+  int n, dx, H, lp_log;                 // lp_log: log2 of the lanes a pair takes
+  // forward out
+  void* Y;
+  float *wV, *S, *stat;                 // S (B,n,n,H) and stat (B,n,H,2) = {max, 1 / sum}: nullable (no backward wanted)
+  uint8_t *q1, *q1s;                    // 8-bit copy of E1: nullable
+  // backward
+  const void* dY;
+  const float* dwV;
+  float *dQp, *dKp, *dVp;               // (jchunks, B, n, dx), (iblocks, B, n, dx) x 2
+  void *dE1, *dE2;
+  int B, jchunk, njc, nib;
+};
+
+#define OOB 0x80000000u                 // past every descriptor's range (the host keeps ranges below 2^31)
+template <class TE, int C> struct Raw { unsigned w[sizeof(TE) * C / 4]; };
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+}
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+template <int W>
+__device__ __forceinline__ void bld(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned (&w)[W]) {
+  if constexpr (W == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+  else if constexpr (W == 2) { const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); w[0] = v.x; w[1] = v.y; }
+  else {
+#pragma unroll
+    for (int k = 0; k < W / 4; ++k) {
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, 0, 0);
+      w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
+    }
+  }
+}
+template <class TE, int C>
+__device__ __forceinline__ void widen(const Raw<TE, C>& r, float (&v)[C]) {
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    if constexpr (sizeof(TE) == 2) v[k] = k & 1 ? bf16_hi(r.w[k / 2]) : bf16_lo(r.w[k / 2]);
+    else v[k] = __builtin_bit_cast(float, r.w[k]);
+  }
+}
+template <class TE, int C>
+__device__ __forceinline__ void gst(TE* p, const float (&v)[C]) {
+  if constexpr (sizeof(TE) == 2 && C == 8) {
+    *reinterpret_cast<uint4*>(p) = uint4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+  } else if constexpr (sizeof(TE) == 2) {
+    *reinterpret_cast<uint2*>(p) = uint2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int k = 0; k < C; k += 4) *reinterpret_cast<float4*>(p + k) = float4{v[k], v[k + 1], v[k + 2], v[k + 3]};
+  }
+}
+#define DPPF(v, ctrl) __builtin_bit_cast(float, MX8_DPP(__builtin_bit_cast(unsigned, v), ctrl))
+// sum over 2^HLOG neighbouring lanes, in every one of them
+template <int HLOG>
+__device__ __forceinline__ float head_sum(float v) {
+  if constexpr (HLOG >= 1) v += DPPF(v, 0xB1);
+  if constexpr (HLOG >= 2) v += DPPF(v, 0x4E);
+  if constexpr (HLOG >= 3) v += DPPF(v, 0x141);
+  if constexpr (HLOG >= 4) v += DPPF(v, 0x140);
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Forward.  A workgroup owns RW query rows; its 4 waves x 64 / LP key slots walk the keys, each with an online softmax of its own (running
+// maximum, sum, weighted V in registers), merged over the slots by lane exchange and over the waves in LDS.
+template <class TE, int C, int HLOG, int RW, bool SAVE, bool MX8>
+__global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
+  extern __shared__ float s_st[];                                       // [4][RW][dx] weighted V, [4][RW][H][2] maximum, sum
+  const int n = a.n, dx = a.dx, H = a.H;
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
+  const int NS = 64 >> a.lp_log, JS = 4 * NS;
+  const bool act = li * C < dx;
+  const int c = act ? li * C : 0, h = c / (C << HLOG);
+  const int nblk = (n + RW - 1) / RW, b = blockIdx.x / nblk, i0 = (blockIdx.x - b * nblk) * RW;
+  const int rows = min(RW, n - i0);
+  const size_t node0 = (size_t)b * n, row0 = node0 + i0;
+  const uint8_t* nm = a.nm + node0;
+  const int* grp = a.grp ? a.grp + node0 : nullptr;
+  const unsigned es = sizeof(TE);
+  const __amdgpu_buffer_rsrc_t r1 = rsrc((const TE*)a.E1 + row0 * n * dx, rows * n * dx * es), r2 = rsrc((const TE*)a.E2 + row0 * n * dx, rows * n * dx * es);
+  const __amdgpu_buffer_rsrc_t rk = rsrc(a.K + node0 * dx, n * dx * 4), rv = rsrc(a.V + node0 * dx, n * dx * 4);
+  const __amdgpu_buffer_rsrc_t rq = rsrc(a.Q + row0 * dx, rows * dx * 4);
+  float q[RW][C], acc[RW][C], m[RW], l[RW];
+  bool mi[RW];
+  int gi[RW];
+#pragma unroll
+  for (int t = 0; t < RW; ++t) {
+    Raw<float, C> rw;
+    bld(rq, act ? (t * dx + c) * 4 : OOB, rw.w);
+    widen(rw, q[t]);
+    const int i = min(i0 + t, n - 1);
+    mi[t] = nm[i] != 0;
+    gi[t] = grp ? grp[i] : 0;
+    m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; ++k) { q[t][k] *= a.qscale; acc[t][k] = 0.f; }
+  }
+  const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+  Raw<TE, C> e1n[RW], e2n[RW];
+  Raw<float, C> kn, vn;
+  // node flags of a key two steps ahead of its use: they decide the addresses of the next step's loads
+  struct Meta { uint8_t m; int g; };
+  auto meta = [&](int j) { const int jc = min(j, n - 1); return Meta{nm[jc], grp ? grp[jc] : 0}; };
+  auto fetch = [&](int j, Meta f) {
+    const unsigned ko = act && j < n ? (unsigned)(j * dx + c) * 4 : OOB;
+    bld(rk, ko, kn.w); bld(rv, ko, vn.w);
+#pragma unroll
+    for (int t = 0; t < RW; ++t) {
+      const unsigned eo = act && j < n && f.m != 0 && mi[t] ? (unsigned)((t * n + j) * dx + c) * es : OOB;
+      bld(r1, eo, e1n[t].w); bld(r2, eo, e2n[t].w);
+    }
+  };
+  const int jf = w * NS + slot;
+  Meta f0 = meta(jf), f1 = meta(jf + JS);
+  fetch(jf, f0);
+  for (int j0 = 0; j0 < n; j0 += JS) {
+    const int j = j0 + jf;
+    Raw<TE, C> e1r[RW], e2r[RW];
+    float kk[C], vv[C];
+#pragma unroll
+    for (int t = 0; t < RW; ++t) { e1r[t] = e1n[t]; e2r[t] = e2n[t]; }
+    widen(kn, kk); widen(vn, vv);
+    const int gj = j < n ? f0.g : -1;
+    f0 = f1;
+    f1 = meta(j + 2 * JS);
+    fetch(j + JS, f0);
+#pragma unroll
+    for (int t = 0; t < RW; ++t) {
+      const bool st = j < n && t < rows;
+      const size_t pair = (row0 + t) * n + j;
+      float e1[C], e2[C], y[C];
+      widen(e1r[t], e1); widen(e2r[t], e2);
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < C; ++k) { y[k] = (q[t][k] * kk[k]) * (e1[k] + 1.f) + e2[k]; s += y[k]; }
+      if (st && act) gst((TE*)a.Y + pair * dx + c, y);
+      if constexpr (MX8) {
+        unsigned mb = 0;
+#pragma unroll
+        for (int k = 0; k < C; ++k) mb = dpp_max_u32(mb, abs_bits(e1[k]));
+        const unsigned sb = mx8_scale(C == 8 ? quad_max(mb) : oct_max(mb));
+        const float inv = mx8_inv(sb);
+        if (st && act) {
+          unsigned* d = reinterpret_cast<unsigned*>(a.q1 + pair * dx + c);
+          const unsigned w0 = mx8_pack4<false>(e1[0], e1[1], e1[2], e1[3], inv);
+          if constexpr (C == 8) *reinterpret_cast<uint2*>(d) = uint2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)};
+          else *d = w0;
+          if (c % MX8_GROUP == 0) a.q1s[pair * (dx / MX8_GROUP) + c / MX8_GROUP] = (uint8_t)sb;
+        }
+      }
+      s = head_sum<HLOG>(s);
+      if (a.cap > 0.f) s = a.cap * tanhf(s * inv_cap);
+      const bool on = gj >= 0 && gj == gi[t];
+      s = on ? s : -INFINITY;
+      if constexpr (SAVE) {
+        if (st && act && (li & ((1 << HLOG) - 1)) == 0) a.S[pair * H + h] = s;
+      }
+      const float mx = fmaxf(m[t], s), mg = mx == -INFINITY ? 0.f : mx;
+      const float sc = __expf(m[t] - mg), p = on ? __expf(s - mg) : 0.f;
+      m[t] = mx;
+      l[t] = l[t] * sc + p;
+#pragma unroll
+      for (int k = 0; k < C; ++k) acc[t][k] = acc[t][k] * sc + p * (on ? vv[k] : 0.f);
+    }
+  }
+  for (int off = 1 << a.lp_log; off < 64; off <<= 1)                    // the key slots of the wave
+#pragma unroll
+    for (int t = 0; t < RW; ++t) {
+      const float mo = __shfl_xor(m[t], off), M = fmaxf(m[t], mo), mg = M == -INFINITY ? 0.f : M;
+      const float x = __expf(m[t] - mg), y = __expf(mo - mg);
+      l[t] = l[t] * x + __shfl_xor(l[t], off) * y;
+      m[t] = M;
+#pragma unroll
+      for (int k = 0; k < C; ++k) acc[t][k] = acc[t][k] * x + __shfl_xor(acc[t][k], off) * y;
+    }
+  float* s_ml = s_st + 4 * RW * dx;
+  if (slot == 0 && act) {
+#pragma unroll
+    for (int t = 0; t < RW; ++t) {
+      gst(s_st + (w * RW + t) * dx + c, acc[t]);
+      if ((li & ((1 << HLOG) - 1)) == 0) { s_ml[((w * RW + t) * H + h) * 2] = m[t]; s_ml[((w * RW + t) * H + h) * 2 + 1] = l[t]; }
+    }
+  }
+  __syncthreads();
+  const int df = C << HLOG;
+  for (int u = threadIdx.x; u < rows * dx; u += 256) {
+    const int t = u / dx, cc = u - t * dx, hh = cc / df;
+    float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, s_ml[((k * RW + t) * H + hh) * 2]);
+    const float mg = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float x = __expf(s_ml[((k * RW + t) * H + hh) * 2] - mg);
+      L += s_ml[((k * RW + t) * H + hh) * 2 + 1] * x; A += s_st[(k * RW + t) * dx + cc] * x;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;                         // no key: 0
+    a.wV[(row0 + t) * dx + cc] = L == 0.f ? 0.f : A * inv;
+    if (SAVE && cc % df == 0) *reinterpret_cast<float2*>(a.stat + ((row0 + t) * H + hh) * 2) = float2{mg, inv};
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Backward.  A workgroup of NW waves owns NW RW query rows (RW a wave) and a chunk of keys; its waves take the same keys at the same time, so dK_j
+// and dV_j are summed over the workgroup's rows in registers and LDS, and only one partial result per NW RW rows reaches memory.  dQ
+// stays in registers over the chunk.  k_attn_head_fold adds the partial results in order (no atomics: the sums do not depend on timing).
+#define HEAD_NW 8
+#define HEAD_RW 2
+template <class TY, int C, int HLOG, bool MX8>
+__global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
+  constexpr int RW = HEAD_RW, NW = HEAD_NW;
+  extern __shared__ float s_kv[];                                       // [2][NW][NS][2][dx]
+  const int n = a.n, dx = a.dx, H = a.H;
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
+  const int NS = 64 >> a.lp_log;
+  const bool act = li * C < dx;
+  const int c = act ? li * C : 0, h = c / (C << HLOG);
+  const int jc = blockIdx.x % a.njc, ib = (blockIdx.x / a.njc) % a.nib, b = blockIdx.x / a.njc / a.nib;
+  const int i0 = (ib * NW + w) * RW, rows = max(0, min(RW, n - i0));
+  const int j_lo = jc * a.jchunk, j_hi = min(n, j_lo + a.jchunk);
+  const size_t node0 = (size_t)b * n, row0 = node0 + min(i0, n - 1);
+  const uint8_t* nm = a.nm + node0;
+  const unsigned es = sizeof(TY), range = (unsigned)(rows * n) * dx;
+  const __amdgpu_buffer_rsrc_t r1 = MX8 ? rsrc((const uint8_t*)a.E1 + row0 * n * dx, range) : rsrc((const TY*)a.E1 + row0 * n * dx, range * es);
+  const __amdgpu_buffer_rsrc_t rsc = rsrc(MX8 ? a.E1s + row0 * n * (dx / MX8_GROUP) : nullptr, MX8 ? range / MX8_GROUP : 0);
+  const __amdgpu_buffer_rsrc_t ry = rsrc((const TY*)a.dY + row0 * n * dx, range * es);
+  const __amdgpu_buffer_rsrc_t rS = rsrc(a.S + row0 * n * H, rows * n * H * 4);
+  const __amdgpu_buffer_rsrc_t rk = rsrc(a.K + node0 * dx, n * dx * 4), rv = rsrc(a.V + node0 * dx, n * dx * 4);
+  const __amdgpu_buffer_rsrc_t rq = rsrc(a.Q + row0 * dx, rows * dx * 4), ro = rsrc(a.wV + row0 * dx, rows * dx * 4), rg = rsrc(a.dwV + row0 * dx, rows * dx * 4);
+  float q[RW][C], g[RW][C], dq[RW][C], D[RW], mx[RW], il[RW];
+  bool mi[RW];
+#pragma unroll
+  for (int t = 0; t < RW; ++t) {
+    const unsigned off = act ? (unsigned)(t * dx + c) * 4 : OOB;        // rows past the end: zeros throughout
+    Raw<float, C> x;
+    bld(rq, off, x.w); widen(x, q[t]);
+    bld(rg, off, x.w); widen(x, g[t]);
+    float o[C], d = 0.f;
+    bld(ro, off, x.w); widen(x, o);
+#pragma unroll
+    for (int k = 0; k < C; ++k) { d += g[t][k] * o[k]; q[t][k] *= a.qscale; dq[t][k] = 0.f; }
+    D[t] = head_sum<HLOG>(d);
+    const int i = min(i0 + t, n - 1);
+    mi[t] = t < rows && nm[i] != 0;
+    const float2 st = *reinterpret_cast<const float2*>(a.stat + ((node0 + i) * H + h) * 2);
+    mx[t] = t < rows ? st.x : 0.f; il[t] = t < rows ? st.y : 0.f;
+  }
+  const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+  constexpr int W1 = MX8 ? C / 4 : (int)sizeof(TY) * C / 4;
+  struct Ops { unsigned e1[W1], sc, s; Raw<TY, C> dy; };
+  Ops nx[RW];
+  Raw<float, C> kn, vn;
+  auto meta = [&](int j) { return nm[min(j, n - 1)]; };
+  auto fetch = [&](int j, uint8_t mj) {
+    const bool on = act && j < j_hi;
+    const unsigned ko = on ? (unsigned)(j * dx + c) * 4 : OOB;
+    bld(rk, ko, kn.w); bld(rv, ko, vn.w);
+#pragma unroll
+    for (int t = 0; t < RW; ++t) {
+      const unsigned p = (unsigned)(t * n + j), e = p * dx + c;
+      const bool pm = on && mj != 0 && mi[t];
+      bld(r1, pm ? (MX8 ? e : e * es) : OOB, nx[t].e1);
+      if constexpr (MX8) nx[t].sc = __builtin_amdgcn_raw_buffer_load_b8(rsc, pm ? p * (dx / MX8_GROUP) + c / MX8_GROUP : OOB, 0, 0);
+      bld(ry, on ? e * es : OOB, nx[t].dy.w);
+      nx[t].s = __builtin_amdgcn_raw_buffer_load_b32(rS, on ? (p * H + h) * 4 : OOB, 0, 0);
+    }
+  };
+  uint8_t m0 = meta(j_lo + slot), m1 = meta(j_lo + slot + NS);
+  fetch(j_lo + slot, m0);
+  int buf = 0;
+  for (int j0 = j_lo; j0 < j_hi; j0 += NS, buf ^= 1) {
+    const int j = j0 + slot;
+    Ops cu[RW];
+    float kk[C], vv[C], dk[C], dv[C];
+#pragma unroll
+    for (int t = 0; t < RW; ++t) cu[t] = nx[t];
+    widen(kn, kk); widen(vn, vv);
+    const bool mj = j < j_hi && m0 != 0;
+    m0 = m1;
+    m1 = meta(j + 2 * NS);
+    fetch(j + NS, m0);
+#pragma unroll
+    for (int k = 0; k < C; ++k) dk[k] = dv[k] = 0.f;
+#pragma unroll
+    for (int t = 0; t < RW; ++t) {
+      float e1[C], G[C], o1[C], o2[C], dp = 0.f;
+      if constexpr (MX8) {
+        const float step = mx8_step(cu[t].sc < MX8_B_MIN ? MX8_B_MIN : cu[t].sc);          // (a masked pair reads 0)
+#pragma unroll
+        for (int k = 0; k < C; k += 4) {
+          e1[k] = mx8_elem<0>(cu[t].e1[k / 4]) * step; e1[k + 1] = mx8_elem<1>(cu[t].e1[k / 4]) * step;
+          e1[k + 2] = mx8_elem<2>(cu[t].e1[k / 4]) * step; e1[k + 3] = mx8_elem<3>(cu[t].e1[k / 4]) * step;
+        }
+      } else {
+        Raw<TY, C> r;
+#pragma unroll
+        for (int k = 0; k < W1; ++k) r.w[k] = cu[t].e1[k];
+        widen(r, e1);
+      }
+      widen(cu[t].dy, G);
+#pragma unroll
+      for (int k = 0; k < C; ++k) dp += g[t][k] * vv[k];
+      dp = head_sum<HLOG>(dp);
+      const float s = __builtin_bit_cast(float, cu[t].s), cs = s * inv_cap;
+      const bool on = t < rows && j < j_hi && s != -INFINITY;
+      const float p = on ? __expf(s - mx[t]) * il[t] : 0.f;
+      const float ds = on ? p * (dp - D[t]) * (1.f - cs * cs) : 0.f;
+      const bool pm = mj && mi[t];
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        G[k] += ds;
+        o2[k] = pm ? G[k] : 0.f;
+        o1[k] = o2[k] * (q[t][k] * kk[k]);
+        const float x = G[k] * (e1[k] + 1.f);
+        dq[t][k] += x * kk[k];
+        dk[k] += x * q[t][k];
+        dv[k] += p * g[t][k];
+      }
+      if (t < rows && j < j_hi && act) {
+        const size_t e = ((row0 + t) * n + j) * dx + c;
+        gst((TY*)a.dE1 + e, o1); gst((TY*)a.dE2 + e, o2);
+      }
+    }
+    float* mine = s_kv + (((buf * NW + w) * NS + slot) * 2) * dx + c;
+    if (act) { gst(mine, dk); gst(mine + dx, dv); }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");     // LDS only: the global loads in flight stay in flight
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    // the waves' sums; the other buffer is written next, and this one again only after the barrier that follows this read
+    const int quads = 2 * dx / 4;
+    for (int u = threadIdx.x; u < NS * quads; u += 64 * NW) {
+      const int sl = u / quads, cq = u - sl * quads;
+      const float* src = s_kv + ((buf * NW * NS + sl) * 2) * dx + cq * 4;
+      float4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(src + (size_t)k * NS * 2 * dx);
+        t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+      }
+      const int cc = cq * 4 < dx ? cq * 4 : cq * 4 - dx;
+      float* dst = (cq * 4 < dx ? a.dKp : a.dVp) + (((size_t)ib * a.B + b) * n + j0 + sl) * dx + cc;
+      if (j0 + sl < j_hi) *reinterpret_cast<float4*>(dst) = t;
+    }
+  }
+  for (int off = 1 << a.lp_log; off < 64; off <<= 1)
+#pragma unroll
+    for (int t = 0; t < RW; ++t)
+#pragma unroll
+      for (int k = 0; k < C; ++k) dq[t][k] += __shfl_xor(dq[t][k], off);
+  if (slot == 0 && act)
+#pragma unroll
+    for (int t = 0; t < RW; ++t)
+      if (t < rows) {
+#pragma unroll
+        for (int k = 0; k < C; ++k) dq[t][k] *= a.qscale;
+        gst(a.dQp + (((size_t)jc * a.B + b) * n + i0 + t) * dx + c, dq[t]);
+      }
+}
+// partial results in order: dQ over the key chunks, dK and dV over the row blocks
+__global__ void __launch_bounds__(256) k_attn_head_fold(const float4* __restrict__ pQ, const float4* __restrict__ pK, const float4* __restrict__ pV,
+                                                        float4* __restrict__ dQ, float4* __restrict__ dK, float4* __restrict__ dV, int njc, int nib,
+                                                        long long quads) {
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (t >= quads) return;
+  const int which = blockIdx.y + (njc > 1 ? 0 : 1);                     // what has one partial result is in place already
+  const float4* src = which == 0 ? pQ : which == 1 ? pK : pV;
+  const int G = which == 0 ? njc : nib;
+  float4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < G; ++g) {
+    const float4 x = src[(size_t)g * quads + t];
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  (which == 0 ? dQ : which == 1 ? dK : dV)[t] = s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// channels per lane and lanes per head; false: not built
+static bool head_shape(int dx, int H, int* C, int* hlog, int* lp_log) {
+  if (dx < 4 || H < 1 || dx % H) return false;
+  const int df = dx / H;
+  *C = df == 4 ? 4 : 8;
+  int l = 0;
+  while ((*C << l) < df) ++l;
+  if ((*C << l) != df || l > 4 || dx / *C > 64) return false;
+  *hlog = l;
+  int p = 0;
+  while ((1 << p) < dx / *C) ++p;
+  *lp_log = p;
+  return true;
+}
+// backward: the row blocks and the keys' chunks: enough workgroups to fill the chip (2 per CU), chunks of at least 8 steps
+static void head_chunks(int B, int n, int lp_log, int* nib, int* njc, int* jchunk) {
+  const int NS = 64 >> lp_log;
+  *nib = (n + HEAD_NW * HEAD_RW - 1) / (HEAD_NW * HEAD_RW);
+  const long long have = (long long)B * *nib;
+  int want = (int)((512 + have - 1) / have);
+  const int most = (n + 8 * NS - 1) / (8 * NS);
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  *jchunk = (n + want - 1) / want;
+  *jchunk = (*jchunk + NS - 1) / NS * NS;
+  *njc = (n + *jchunk - 1) / *jchunk;
+}
+
+template <class TE, int C, int HLOG>
+static void fwd_launch(const HeadArgs& a, bool save, bool mx8, hipStream_t s) {
+  constexpr int WIDE = sizeof(TE) == 2 ? 4 : 2;                         // rows per workgroup where that still gives 2 workgroups per CU, else 1
+  const bool wide = (long long)a.B * ((a.n + WIDE - 1) / WIDE) >= 512;
+  const int RW = wide ? WIDE : 1;
+  const long long grid = (long long)a.B * ((a.n + RW - 1) / RW);
+  const size_t lds = sizeof(float) * 4 * RW * (a.dx + 2 * a.H);
+#define F(R, S, M) k_attn_head_fwd<TE, C, HLOG, R, S, M><<<(unsigned)grid, 256, lds, s>>>(a)
+  if (wide) { if (mx8) F(WIDE, true, true); else if (save) F(WIDE, true, false); else F(WIDE, false, false); }
+  else { if (mx8) F(1, true, true); else if (save) F(1, true, false); else F(1, false, false); }
+#undef F
+}
+template <class TY, int C, int HLOG>
+static void bwd_launch(const HeadArgs& a, bool mx8, hipStream_t s) {
+  const unsigned grid = (unsigned)((long long)a.B * a.nib * a.njc);
+  const size_t lds = sizeof(float) * 2 * HEAD_NW * (64 >> a.lp_log) * 2 * a.dx;             // 64 KB at most
+  if (mx8) k_attn_head_bwd<TY, C, HLOG, true><<<grid, 64 * HEAD_NW, lds, s>>>(a);
+  else k_attn_head_bwd<TY, C, HLOG, false><<<grid, 64 * HEAD_NW, lds, s>>>(a);
+}
+template <class T, class F>
+static void by_shape(int C, int hlog, F f) {
+  if (C == 4) f(std::integral_constant<int, 4>{}, std::integral_constant<int, 0>{});
+  else switch (hlog) {
+    case 0: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 0>{}); break;
+    case 1: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{}); break;
+    case 3: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 3>{}); break;
+    default: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}); break;
+  }
+}
+static bool al16(std::initializer_list<const void*> ps) {
+  uintptr_t v = 0;
+  for (const void* p : ps) v |= (uintptr_t)p;
+  return (v & 15) == 0;
+}
+// sizes both passes take: the descriptors' ranges and offsets are 32-bit (4 rows of a graph's pairs), the grid one-dimensional
+static int head_sizes(const char* who, int B, int n, int dx, int H, int* C, int* hlog, int* lp_log) {
+  DA_CHECK_ARG(B >= 0 && n >= 0 && dx >= 1 && H >= 1, "%s: B = %d, n = %d, dx = %d, n_head = %d", who, B, n, dx, H);
+  if (!head_shape(dx, H, C, hlog, lp_log)) {
+    da_set_error("%s: dx = %d with %d heads not built (channels per head 4, 8, 16, .. 128; dx <= 512, 256 with 4 channels per head)", who, dx, H);
+    return DA_ERR_UNSUPPORTED;
+  }
+  DA_CHECK_ARG(4LL * n * dx * 4 < (1LL << 31) && 16LL * n * H < (1LL << 31) && (long long)B * n < (1LL << 31), "%s: B = %d, n = %d too large", who, B, n);
+  return DA_OK;
+}
+
+extern "C" {
+
+int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void* E1, const void* E2, int e_bf16, const uint8_t* node_mask,
+                     const int* groups, float qscale, float cap, void* Y, float* wV, float* S, float* stat, void* E1_codes, uint8_t* E1_scales, int B,
+                     int n, int dx, int n_head, void* stream) {
+  HeadArgs a = {};
+  int C, hlog;
+  if (int rc = head_sizes("da_attn_head_fwd", B, n, dx, n_head, &C, &hlog, &a.lp_log)) return rc;
+  if (B == 0 || n == 0) return DA_OK;
+  DA_CHECK_ARG(Q && K && V && E1 && E2 && node_mask && Y && wV, "da_attn_head_fwd: null pointer");
+  DA_CHECK_ARG((S == nullptr) == (stat == nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr) && (!E1_codes || S),
+               "da_attn_head_fwd: S and stat go together, E1's codes and scales with both");
+  DA_CHECK_ARG(!E1_codes || dx % MX8_GROUP == 0, "da_attn_head_fwd: 8-bit E1 needs dx %% 32 == 0, dx = %d", dx);
+  DA_CHECK_ARG(cap >= 0.f && cap < INFINITY, "da_attn_head_fwd: cap = %g", cap);
+  DA_CHECK_ARG(al16({Q, K, V, E1, E2, Y, wV, S, stat, E1_codes}), "da_attn_head_fwd: unaligned tensor (16 bytes)");
+  a.Q = Q; a.K = K; a.V = V; a.E1 = E1; a.E2 = E2; a.nm = node_mask; a.grp = groups; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx; a.H = n_head;
+  a.Y = Y; a.wV = wV; a.S = S; a.stat = stat; a.q1 = (uint8_t*)E1_codes; a.q1s = E1_scales; a.B = B;
+  by_shape<void>(C, hlog, [&](auto c, auto h) {
+    if (e_bf16) fwd_launch<bf16_t, decltype(c)::value, decltype(h)::value>(a, S != nullptr, E1_codes != nullptr, (hipStream_t)stream);
+    else fwd_launch<float, decltype(c)::value, decltype(h)::value>(a, S != nullptr, E1_codes != nullptr, (hipStream_t)stream);
+  });
+  DA_CHECK_LAUNCH("da_attn_head_fwd");
+  return DA_OK;
+}
+
+long long da_attn_head_bwd_workspace(int B, int n, int dx, int n_head) {
+  int C, hlog, lp, nib, njc, jchunk;
+  if (B < 0 || n < 0 || !head_shape(dx, n_head, &C, &hlog, &lp)) return -1;
+  if (B == 0 || n == 0) return 0;
+  head_chunks(B, n, lp, &nib, &njc, &jchunk);
+  return (long long)sizeof(float) * ((nib > 1 ? 2LL * nib : 0) + (njc > 1 ? njc : 0)) * B * n * dx;
+}
+
+int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void* E1, const void* E1_codes, const uint8_t* E1_scales,
+                     const uint8_t* node_mask, float qscale, float cap, const float* wV, const float* S, const float* stat, const void* dY,
+                     int dy_bf16, const float* dwV, float* dQ, float* dK, float* dV, void* dE1, void* dE2, void* workspace,
+                     long long workspace_bytes, int B, int n, int dx, int n_head, void* stream) {
+  HeadArgs a = {};
+  int C, hlog;
+  if (int rc = head_sizes("da_attn_head_bwd", B, n, dx, n_head, &C, &hlog, &a.lp_log)) return rc;
+  if (B == 0 || n == 0) return DA_OK;
+  DA_CHECK_ARG(Q && K && V && node_mask && wV && S && stat && dY && dwV && dQ && dK && dV && dE1 && dE2, "da_attn_head_bwd: null pointer");
+  DA_CHECK_ARG((E1 != nullptr) != (E1_codes != nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr),
+               "da_attn_head_bwd: E1 either at full width or as codes and scales");
+  DA_CHECK_ARG(!E1_codes || dx % MX8_GROUP == 0, "da_attn_head_bwd: 8-bit E1 needs dx %% 32 == 0, dx = %d", dx);
+  DA_CHECK_ARG(cap >= 0.f && cap < INFINITY, "da_attn_head_bwd: cap = %g", cap);
+  DA_CHECK_ARG(al16({Q, K, V, E1, E1_codes, wV, S, stat, dY, dwV, dQ, dK, dV, dE1, dE2, workspace}), "da_attn_head_bwd: unaligned tensor (16 bytes)");
+  const long long need = da_attn_head_bwd_workspace(B, n, dx, n_head);
+  DA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "da_attn_head_bwd: workspace too small");
+  a.Q = Q; a.K = K; a.V = V; a.E1 = E1_codes ? E1_codes : E1; a.E1s = E1_scales; a.nm = node_mask; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx;
+  a.H = n_head; a.wV = (float*)wV; a.S = (float*)S; a.stat = (float*)stat; a.dY = dY; a.dwV = dwV; a.dE1 = dE1; a.dE2 = dE2; a.B = B;
+  head_chunks(B, n, a.lp_log, &a.nib, &a.njc, &a.jchunk);
+  const size_t one = (size_t)B * n * dx;
+  float* ws = (float*)workspace;
+  a.dKp = dK; a.dVp = dV; a.dQp = dQ;
+  if (a.nib > 1) { a.dKp = ws; a.dVp = ws + a.nib * one; ws += 2 * a.nib * one; }
+  if (a.njc > 1) a.dQp = ws;
+  hipStream_t s = (hipStream_t)stream;
+  by_shape<void>(C, hlog, [&](auto c, auto h) {
+    if (dy_bf16) bwd_launch<bf16_t, decltype(c)::value, decltype(h)::value>(a, E1_codes != nullptr, s);
+    else bwd_launch<float, decltype(c)::value, decltype(h)::value>(a, E1_codes != nullptr, s);
+  });
+  if (a.nib > 1 || a.njc > 1) {
+    const long long quads = (long long)one / 4;
+    const unsigned gx = (unsigned)((quads + 255) / 256);
+    k_attn_head_fold<<<dim3(gx, (a.njc > 1 ? 1 : 0) + (a.nib > 1 ? 2 : 0)), 256, 0, s>>>((const float4*)a.dQp, (const float4*)a.dKp, (const float4*)a.dVp, (float4*)dQ, (float4*)dK,
+                                                                 (float4*)dV, a.njc, a.nib, quads);
+  }
+  DA_CHECK_LAUNCH("da_attn_head_bwd");
+  return DA_OK;
+}
+
+}  // extern "C"

@@ -193,6 +193,24 @@ int da_res_ln_bwd(const float* s, const float* gamma, const float* d_out, const 
  * backward: dx = dy / (1 - p) where the stored result is non-zero, else 0 (no mask kept; dx may alias dy). */
 int da_relu_dropout(void* h, int is_bf16, long long numel, const long long* seed, int salt, float p, void* stream);
 int da_relu_dropout_bwd(const void* h, const void* dy, void* dx, int is_bf16, long long numel, float p, void* stream);
+/* ---- per-head edge attention (NodeEdgeBlockImproved, neuralnet/layers.py:115-141), forward and backward.  m_ij = m_i m_j:
+ *   Y = qscale Q_i K_j (1 + m_ij E1) + m_ij E2 (the input of e_out);  S = sum of Y over a head's dx / n_head channels, cap tanh(S / cap) with
+ *   cap > 0;  wV = softmax over keys of S times V.  groups (B,n) int32 (NULL: all keys, as the reference): row i sees the keys with
+ *   groups[j] == groups[i] >= 0; a row without a key gets wV = 0.  E1 and E2 are not read where m_ij = 0.
+ * Q, K, V, wV (B,n,dx) fp32; E1, E2, Y (B,n,n,dx) fp32 or bf16 (e_bf16).  For a backward: S (B,n,n,n_head) fp32 and stat (B,n,n_head,2) are
+ * written when given (both or neither), and E1_codes / E1_scales get E1 in 8 bits (da_mx8_quant's format; dx % 32 == 0).
+ * Built: 4, 8, 16, .. 128 channels per head, dx <= 512 (256 with 4 channels per head); others: DA_ERR_UNSUPPORTED.  16-byte aligned tensors. */
+int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void* E1, const void* E2, int e_bf16, const uint8_t* node_mask,
+                     const int* groups, float qscale, float cap, void* Y, float* wV, float* S, float* stat, void* E1_codes, uint8_t* E1_scales, int B,
+                     int n, int dx, int n_head, void* stream);
+/* From dY (B,n,n,dx) fp32 or bf16 (dy_bf16) and dwV (B,n,dx) to dQ, dK, dV fp32, dE1, dE2 of dY's type (0 where m_ij = 0).  E1 of dY's type, or
+ * NULL with its codes and scales.  wV, S, stat as the forward left them; workspace (da_attn_head_bwd_workspace bytes, -1: not built) holds
+ * partial dQ, dK, dV, folded in order (deterministic). */
+long long da_attn_head_bwd_workspace(int B, int n, int dx, int n_head);
+int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void* E1, const void* E1_codes, const uint8_t* E1_scales,
+                     const uint8_t* node_mask, float qscale, float cap, const float* wV, const float* S, const float* stat, const void* dY,
+                     int dy_bf16, const float* dwV, float* dQ, float* dK, float* dV, void* dE1, void* dE2, void* workspace,
+                     long long workspace_bytes, int B, int n, int dx, int n_head, void* stream);
 /* ---- 8-bit activation checkpoints of the training step (the reference keeps full-width activations for loss.backward(),
  * training/helpers.py:139-142).  MXINT8: 32 consecutive channels of a row share the scale 2^(b-127) (one byte b), an element is an int8 q and
  * stands for q / 64 * 2^(b-127); b is the smallest in [27, 254] at which the group's largest magnitude rounds to 127 or less, 255 (codes 0: the
