@@ -208,45 +208,53 @@ class AttnCoreBF16(Function):
 
 class HeadAttnCore(Function):
     """The core of NodeEdgeBlockImproved (layers.py:115-141) between the q/k/v/e_mul/e_add projections and e_out / the y_x FiLM; called through
-    head_attention.  `save`: leave the scores and softmax statistics for the backward, and E1 as `checkpoint` says ('none': as it is,
-    'mx8': 8 bits, written by the forward kernel while it reads E1)."""
+    head_attention, which checks and prepares the arguments.  `save`: leave the scores and softmax statistics for the backward, and E1 as
+    `mx` says (False: as it is, True: 8 bits, written by the forward kernel while it reads E1)."""
 
     @staticmethod
-    def forward(ctx, Q, K, V, E1, E2, nm_u8, groups, n_head, qscale, cap, checkpoint, save):
+    def forward(ctx, Q, K, V, E1, E2, nm_u8, groups, n_head, qscale, cap, mx, save):
         B, n, dx = Q.shape
         dev = Q.device
         Y, wV = torch.empty_like(E1), torch.empty_like(Q)
-        S = st = codes = scales = None
+        sp = tp = cp = kp = 0
         if save:
-            S, st = torch.empty(B, n, n, n_head, device=dev), torch.empty(B, n, n_head, 2, device=dev)
-            if checkpoint == 'mx8':
+            # statistics (B,n,H,2) and scores (B,n,n,H) in one allocation
+            st = torch.empty(B * n * (n + 2) * n_head, device=dev)
+            tp = st.data_ptr()
+            sp = tp + 8 * B * n * n_head
+            if mx:
                 codes = torch.empty(E1.shape, dtype=torch.int8, device=dev)
-                scales = torch.empty(B, n, n, dx // mx8.GROUP, dtype=torch.uint8, device=dev)
-        with mx8.on_device_of(Q):
-            L.check(L.lib().da_attn_head_fwd(L.ptr(Q), L.ptr(K), L.ptr(V), L.ptr(E1), L.ptr(E2), int(E1.dtype == torch.bfloat16), L.ptr(nm_u8),
-                                             L.ptr(groups), qscale, cap, L.ptr(Y), L.ptr(wV), L.ptr(S), L.ptr(st), L.ptr(codes), L.ptr(scales), B, n, dx,
-                                             n_head, L.stream()), 'da_attn_head_fwd')
-        if save:
-            ctx.save_for_backward(Q, K, V, nm_u8, wV, S, st, *((E1,) if codes is None else (codes, scales)))
-            ctx.meta = (n_head, qscale, cap)
+                scales = torch.empty((B, n, n, dx // mx8.GROUP), dtype=torch.uint8, device=dev)
+                cp, kp = codes.data_ptr(), scales.data_ptr()
+            # (the tensors behind the addresses are locals until the call returns)
+            ctx.save_for_backward(Q, K, V, nm_u8, wV, st, *((codes, scales) if mx else (E1,)))
+            ctx.meta = (n_head, qscale, cap, mx)
+        L.check(L.lib().da_attn_head_fwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), E1.data_ptr(), E2.data_ptr(), E1.dtype is torch.bfloat16,
+                                         nm_u8.data_ptr(), 0 if groups is None else groups.data_ptr(), qscale, cap, Y.data_ptr(), wV.data_ptr(), sp, tp,
+                                         cp, kp, B, n, dx, n_head, L.stream()), 'da_attn_head_fwd')
         return Y, wV
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dY, dwV):
-        Q, K, V, nm_u8, wV, S, st, *e1 = ctx.saved_tensors
-        n_head, qscale, cap = ctx.meta
+        Q, K, V, nm_u8, wV, st, E1, *scales = ctx.saved_tensors
+        if mx8.elsewhere(Q):
+            with torch.cuda.device(Q.device):
+                return HeadAttnCore.backward(ctx, dY, dwV)
+        n_head, qscale, cap, mx = ctx.meta
         B, n, dx = Q.shape
-        dY, dwV = mx8._aligned(dY), _c16(dwV)
-        E1, codes, scales = (e1[0], None, None) if len(e1) == 1 else (None, *e1)
+        dY, dwV = mx8.aligned(dY), mx8.aligned(dwV)
         dQ, dK, dV = torch.empty_like(Q), torch.empty_like(Q), torch.empty_like(Q)
         dE1, dE2 = torch.empty_like(dY), torch.empty_like(dY)
-        with mx8.on_device_of(Q):
-            # the workspace is this call's own: two captured graphs that are replayed side by side must not share one
-            ws = torch.empty(L.lib().da_attn_head_bwd_workspace(B, n, dx, n_head), dtype=torch.uint8, device=Q.device)
-            L.check(L.lib().da_attn_head_bwd(L.ptr(Q), L.ptr(K), L.ptr(V), L.ptr(E1), L.ptr(codes), L.ptr(scales), L.ptr(nm_u8), qscale, cap, L.ptr(wV),
-                                             L.ptr(S), L.ptr(st), L.ptr(dY), int(dY.dtype == torch.bfloat16), L.ptr(dwV), L.ptr(dQ), L.ptr(dK), L.ptr(dV),
-                                             L.ptr(dE1), L.ptr(dE2), L.ptr(ws), ws.numel(), B, n, dx, n_head, L.stream()), 'da_attn_head_bwd')
+        lib = L.lib()
+        nbytes = lib.da_attn_head_bwd_workspace(B, n, dx, n_head)
+        # the workspace is this call's own: two captured graphs that are replayed side by side must not share one
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
+        e1, tp = E1.data_ptr(), st.data_ptr()
+        L.check(lib.da_attn_head_bwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), 0 if mx else e1, e1 if mx else 0, scales[0].data_ptr() if mx else 0,
+                                     nm_u8.data_ptr(), qscale, cap, wV.data_ptr(), tp + 8 * B * n * n_head, tp, dY.data_ptr(), dY.dtype is torch.bfloat16,
+                                     dwV.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dE1.data_ptr(), dE2.data_ptr(), ws.data_ptr(), nbytes,
+                                     B, n, dx, n_head, L.stream()), 'da_attn_head_bwd')
         return dQ, dK, dV, dE1, dE2, None, None, None, None, None, None, None
 
 
@@ -266,15 +274,17 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
     (B,n) integers over the keys of the query's own group (a node with a negative group is in none: its wV is 0, and so is the wV of
     every row without a key).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
     fp32 arithmetic throughout; sums do not depend on timing."""
-    if Q.dim() != 3 or K.shape != Q.shape or V.shape != Q.shape:
-        raise L.DiffAlignHipError(f'head_attention: Q, K, V (B,n,dx) expected, got {tuple(Q.shape)}, {tuple(K.shape)}, {tuple(V.shape)}')
-    B, n, dx = Q.shape
+    shape = Q.shape
+    if len(shape) != 3 or K.shape != shape or V.shape != shape:
+        raise L.DiffAlignHipError(f'head_attention: Q, K, V (B,n,dx) expected, got {tuple(shape)}, {tuple(K.shape)}, {tuple(V.shape)}')
+    B, n, dx = shape
     if E1.shape != (B, n, n, dx) or E2.shape != E1.shape or E1.dtype != E2.dtype or E1.dtype not in (torch.float32, torch.bfloat16):
         raise L.DiffAlignHipError(f'head_attention: E1, E2 {(B, n, n, dx)} of one type, fp32 or bf16, expected, got {E1.dtype} {tuple(E1.shape)}, '
                                   f'{E2.dtype} {tuple(E2.shape)}')
     if node_mask.shape != (B, n) or (groups is not None and (groups.shape != (B, n) or groups.is_floating_point() or groups.dtype == torch.bool)):
         raise L.DiffAlignHipError(f'head_attention: node_mask and groups (integers) of shape {(B, n)} expected')
-    if any(t is not None and t.device != Q.device for t in (K, V, E1, E2, node_mask, groups)):
+    dev = Q.device
+    if not (K.device == dev == V.device and E1.device == dev == E2.device and node_mask.device == dev and (groups is None or groups.device == dev)):
         raise L.DiffAlignHipError('head_attention: tensors on different devices')
     if not head_attention_built(dx, n_head):
         raise L.DiffAlignHipError(f'head_attention: dx = {dx} with {n_head} heads not built')
@@ -285,10 +295,15 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
     cap = float(cap)
     if not 0.0 <= cap < math.inf:
         raise ValueError(f'head_attention: cap = {cap}')
-    save = torch.is_grad_enabled() and any(t.requires_grad for t in (Q, K, V, E1, E2))
-    return HeadAttnCore.apply(_c16(Q), _c16(K), _c16(V), mx8._aligned(E1), mx8._aligned(E2), L.as_u8(node_mask),
-                              None if groups is None else groups.to(torch.int32).contiguous(), n_head,
-                              qscale_of(dx, n_head) if qscale is None else float(qscale), cap, checkpoint, save)
+    mx8.refuse_cpu(Q)
+    if mx8.elsewhere(Q):
+        with torch.cuda.device(dev):
+            return head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale, cap, groups, checkpoint)
+    save = torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad or E1.requires_grad or E2.requires_grad)
+    args = (mx8.aligned(Q.float()), mx8.aligned(K.float()), mx8.aligned(V.float()), mx8.aligned(E1), mx8.aligned(E2), L.as_u8(node_mask),
+            None if groups is None else groups.to(torch.int32).contiguous(), n_head, qscale_of(dx, n_head) if qscale is None else float(qscale), cap,
+            checkpoint == 'mx8', save)
+    return HeadAttnCore.apply(*args) if save else HeadAttnCore.forward(None, *args)
 
 
 class AddLayerNorm(Function):

@@ -10,7 +10,6 @@ The reference keeps every activation at full width for `loss.backward()` (traini
 forward's per-pair Linears and the per-head attention core (train_forward.py, `train_checkpoint = 'mx8'`)."""
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple, Tuple
 
 import torch
@@ -28,20 +27,36 @@ class Mx8(NamedTuple):
     scales: torch.Tensor      # uint8 (..., ceil(D / 32))
 
 
-def on_device_of(t: torch.Tensor):
-    """Launches go to the tensor's device, also where it is not the current one."""
-    return contextlib.nullcontext() if not t.is_cuda or t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+# Host cost: on the small calls (a few thousand rows) the kernels take 3 us and the way to them three times that, so the arguments are checked
+# once here and travel as plain addresses; every tensor behind one is a local of the caller until the entry point has returned.
+def refuse_cpu(t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise L.DiffAlignHipError('diffalign_amd ops need tensors on a HIP device (no CPU fallback); got ' + str(t.device))
+
+
+def elsewhere(t: torch.Tensor) -> bool:
+    """Whether t is on another device than the current one: the caller then runs again with t's device current."""
+    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()
+
+
+def aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
+    """t, contiguous at an address divisible by `to`; itself where it is already."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % to else t
 
 
 def _check(q: Mx8) -> Mx8:
     codes, scales = q
     if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
         raise L.DiffAlignHipError(f'mx8: codes int8 and scales uint8 expected, got {codes.dtype} and {scales.dtype}')
-    if codes.dim() < 1 or scales.shape != codes.shape[:-1] + (-(-codes.shape[-1] // GROUP),):
-        raise L.DiffAlignHipError(f'mx8: scales {tuple(scales.shape)} do not belong to codes {tuple(codes.shape)} (one byte for {GROUP} channels)')
+    shape = codes.shape
+    if len(shape) < 1 or scales.shape != shape[:-1] + (-(-shape[-1] // GROUP),):
+        raise L.DiffAlignHipError(f'mx8: scales {tuple(scales.shape)} do not belong to codes {tuple(shape)} (one byte for {GROUP} channels)')
     if scales.device != codes.device:
         raise L.DiffAlignHipError(f'mx8: codes on {codes.device}, scales on {scales.device}')
-    return Mx8(codes.contiguous(), scales.contiguous())
+    refuse_cpu(codes)
+    return q if codes.is_contiguous() and scales.is_contiguous() else Mx8(codes.contiguous(), scales.contiguous())
 
 
 def quantize(x: torch.Tensor, keep_nonzero: bool = False) -> Mx8:
@@ -50,15 +65,20 @@ def quantize(x: torch.Tensor, keep_nonzero: bool = False) -> Mx8:
     (relu_dropout_bwd)."""
     if x.dtype not in _DTYPES:
         raise L.DiffAlignHipError(f'mx8.quantize: fp32 or bf16 expected, got {x.dtype}')
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise L.DiffAlignHipError(f'mx8.quantize: x needs a channel axis, got shape {tuple(x.shape)}')
-    x = x.detach().contiguous()
-    D = x.shape[-1]
-    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty(x.shape[:-1] + (-(-D // GROUP),), dtype=torch.uint8, device=x.device)
-    with on_device_of(x):
-        L.check(L.lib().da_mx8_quant(L.ptr(x), int(x.dtype == torch.bfloat16), L.ptr(codes), L.ptr(scales), x.numel() // D, D, int(keep_nonzero),
-                                     L.stream()), 'da_mx8_quant')
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise L.DiffAlignHipError(f'mx8.quantize: x needs a channel axis, got shape {tuple(shape)}')
+    refuse_cpu(x)
+    if elsewhere(x):
+        with torch.cuda.device(x.device):
+            return quantize(x, keep_nonzero)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    D = shape[-1]
+    codes = torch.empty(shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(shape[:-1] + (-(-D // GROUP),), dtype=torch.uint8, device=x.device)
+    L.check(L.lib().da_mx8_quant(x.data_ptr(), x.dtype is torch.bfloat16, codes.data_ptr(), scales.data_ptr(), x.numel() // D, D, keep_nonzero, L.stream()),
+            'da_mx8_quant')
     return Mx8(codes, scales)
 
 
@@ -66,54 +86,57 @@ def dequantize(q: Mx8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of an 8-bit activation, fp32 or bf16 (both exact)."""
     if dtype not in _DTYPES:
         raise L.DiffAlignHipError(f'mx8.dequantize: fp32 or bf16, not {dtype}')
-    q = _check(q)
-    D = q.codes.shape[-1]
-    out = torch.empty(q.codes.shape, dtype=dtype, device=q.codes.device)
+    codes, scales = _check(q)
+    if elsewhere(codes):
+        with torch.cuda.device(codes.device):
+            return dequantize(q, dtype)
+    D = codes.shape[-1]
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     if D == 0:
         return out
-    with on_device_of(out):
-        L.check(L.lib().da_mx8_dequant(L.ptr(q.codes), L.ptr(q.scales), L.ptr(out), int(dtype == torch.bfloat16), out.numel() // D, D, L.stream()),
-                'da_mx8_dequant')
+    L.check(L.lib().da_mx8_dequant(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dtype is torch.bfloat16, out.numel() // D, D, L.stream()),
+            'da_mx8_dequant')
     return out
-
-
-def _aligned(t: torch.Tensor, to: int = 16) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % to else t
 
 
 def linear_wgrad(q: Mx8, dy: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(dW (out,in), db (out)) fp32 of an nn.Linear whose input x is held in 8 bits: dW = dY^T x, db = column sums of dY.  dy (..., out)
     fp32 or bf16 with q's leading axes; (in, out) of WGRAD_SHAPES."""
-    q = _check(q)
-    in_f, out_f = q.codes.shape[-1], dy.shape[-1]
+    codes, scales = _check(q)
     if dy.dtype not in _DTYPES:
         raise L.DiffAlignHipError(f'mx8.linear_wgrad: dy fp32 or bf16, got {dy.dtype}')
-    if q.codes.shape[:-1] != dy.shape[:-1] or q.codes.device != dy.device:
-        raise L.DiffAlignHipError(f'mx8.linear_wgrad: x {tuple(q.codes.shape)} on {q.codes.device} and dy {tuple(dy.shape)} on {dy.device} do not belong together')
+    if dy.dim() < 1 or codes.shape[:-1] != dy.shape[:-1] or codes.device != dy.device:
+        raise L.DiffAlignHipError(f'mx8.linear_wgrad: x {tuple(codes.shape)} on {codes.device} and dy {tuple(dy.shape)} on {dy.device} do not belong together')
+    in_f, out_f = codes.shape[-1], dy.shape[-1]
     if (in_f, out_f) not in WGRAD_SHAPES:
         raise L.DiffAlignHipError(f'mx8.linear_wgrad: {in_f} -> {out_f} features not built')
-    R = q.codes.numel() // in_f
-    dW, db = torch.empty(out_f, in_f, device=dy.device), torch.empty(out_f, device=dy.device)
+    if elsewhere(dy):
+        with torch.cuda.device(dy.device):
+            return linear_wgrad(q, dy)
+    R, dev = codes.numel() // in_f, dy.device
+    dW, db = torch.empty(out_f, in_f, device=dev), torch.empty(out_f, device=dev)
     if R == 0:
         return dW.zero_(), db.zero_()
-    codes, dy = _aligned(q.codes, 8), _aligned(dy.detach())
-    with on_device_of(dy):
-        ws = torch.empty(L.lib().da_linear_wgrad_mx8_workspace(R, in_f, out_f), dtype=torch.uint8, device=dy.device)
-        L.check(L.lib().da_linear_wgrad_mx8(L.ptr(codes), L.ptr(q.scales), L.ptr(dy), int(dy.dtype == torch.bfloat16), L.ptr(dW), L.ptr(db), L.ptr(ws),
-                                            ws.numel(), R, in_f, out_f, L.stream()), 'da_linear_wgrad_mx8')
+    codes, dy = aligned(codes, 8), aligned(dy)
+    lib = L.lib()
+    nbytes = lib.da_linear_wgrad_mx8_workspace(R, in_f, out_f)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    L.check(lib.da_linear_wgrad_mx8(codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dy.dtype is torch.bfloat16, dW.data_ptr(), db.data_ptr(),
+                                    ws.data_ptr(), nbytes, R, in_f, out_f, L.stream()), 'da_linear_wgrad_mx8')
     return dW, db
 
 
 def relu_dropout_bwd(q: Mx8, dy: torch.Tensor, p: float) -> torch.Tensor:
     """Gradient of h = dropout_p(relu(a)) with respect to a, from h held in 8 bits with keep_nonzero: dy / (1 - p) where h is not zero,
     else 0.  dy fp32 or bf16, of h's shape."""
-    q = _check(q)
-    if dy.dtype not in _DTYPES or dy.shape != q.codes.shape or dy.device != q.codes.device:
-        raise L.DiffAlignHipError(f'mx8.relu_dropout_bwd: dy fp32 or bf16 of shape {tuple(q.codes.shape)} expected, got {dy.dtype} {tuple(dy.shape)} on {dy.device}')
-    dy = dy.detach().contiguous()
+    codes, _ = _check(q)
+    if dy.dtype not in _DTYPES or dy.shape != codes.shape or dy.device != codes.device:
+        raise L.DiffAlignHipError(f'mx8.relu_dropout_bwd: dy fp32 or bf16 of shape {tuple(codes.shape)} expected, got {dy.dtype} {tuple(dy.shape)} on {dy.device}')
+    if elsewhere(dy):
+        with torch.cuda.device(dy.device):
+            return relu_dropout_bwd(q, dy, p)
+    dy = dy.contiguous()
     dx = torch.empty_like(dy)
-    with on_device_of(dy):
-        L.check(L.lib().da_relu_dropout_bwd_mx8(L.ptr(q.codes), L.ptr(dy), L.ptr(dx), int(dy.dtype == torch.bfloat16), dy.numel(), float(p), L.stream()),
-                'da_relu_dropout_bwd_mx8')
+    L.check(L.lib().da_relu_dropout_bwd_mx8(codes.data_ptr(), dy.data_ptr(), dx.data_ptr(), dy.dtype is torch.bfloat16, dy.numel(), float(p), L.stream()),
+            'da_relu_dropout_bwd_mx8')
     return dx
