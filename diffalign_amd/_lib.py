@@ -45,7 +45,7 @@ SIGNATURES = {
     'da_layernorm_bwd': 'i:pppppppqqip',
     'da_res_ln_fwd': 'i:ppipiipppifpppqip', 'da_res_ln_bwd_workspace': 'q:i', 'da_res_ln_bwd': 'i:pppppiipifppipppqqip',
     'da_relu_dropout': 'i:piqpifp', 'da_relu_dropout_bwd': 'i:pppiqfp',
-    'da_attn_head_fwd': 'i:pppppippff' + 'pppppp' + 'iiiip', 'da_attn_head_bwd_workspace': 'q:iiii',
+    'da_attn_head_fwd': 'i:pppppippff' + 'pppppp' + 'iiiip', 'da_attn_head_bwd_workspace': 'q:iiiii',
     'da_attn_head_bwd': 'i:pppppppff' + 'pppp' + 'ip' + 'ppppp' + 'pq' + 'iiiip',
     'da_mx8_quant': 'i:pippqiip', 'da_mx8_dequant': 'i:pppiqip', 'da_relu_dropout_bwd_mx8': 'i:pppiqfp',
     'da_linear_wgrad_mx8_workspace': 'q:qii', 'da_linear_wgrad_mx8': 'i:pppipppqqiip',

@@ -247,7 +247,7 @@ class HeadAttnCore(Function):
         dQ, dK, dV = torch.empty_like(Q), torch.empty_like(Q), torch.empty_like(Q)
         dE1, dE2 = torch.empty_like(dY), torch.empty_like(dY)
         lib = L.lib()
-        nbytes = lib.da_attn_head_bwd_workspace(B, n, dx, n_head)
+        nbytes = lib.da_attn_head_bwd_workspace(B, n, dx, n_head, dY.dtype is torch.bfloat16)
         # the workspace is this call's own: two captured graphs that are replayed side by side must not share one
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
         e1, tp = E1.data_ptr(), st.data_ptr()

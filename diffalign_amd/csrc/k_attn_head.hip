@@ -21,6 +21,11 @@
 #include <initializer_list>
 #include <type_traits>
 
+// Which product is fused into which sum is written out (fmaf) and left to nobody else: the variants of a kernel then round alike, and the
+// forward gives the same bits with and without a backward to come.
+#pragma clang fp contract(off)
+__device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+
 struct HeadArgs {
   const float *Q, *K, *V;
   const void *E1, *E2;                  // E1: TE, or its codes (8-bit backward)
@@ -41,7 +46,7 @@ struct HeadArgs {
   int B, jchunk, njc, nib;
 };
 
-#define OOB 0x80000000u                 // past every descriptor's range (the host keeps ranges below 2^31)
+#define OOB 0x80000000u                 // past every descriptor's range, also with a row's offset added (the host keeps both below 2^31)
 template <class TE, int C> struct Raw { unsigned w[sizeof(TE) * C / 4]; };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, unsigned bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
@@ -49,13 +54,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, unsigned b
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 template <int W>
-__device__ __forceinline__ void bld(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned (&w)[W]) {
-  if constexpr (W == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-  else if constexpr (W == 2) { const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); w[0] = v.x; w[1] = v.y; }
+__device__ __forceinline__ void bld(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned (&w)[W], unsigned soff = 0) {
+  if constexpr (W == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0);
+  else if constexpr (W == 2) { const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0); w[0] = v.x; w[1] = v.y; }
   else {
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
-      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, 0, 0);
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, soff, 0);
       w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
     }
   }
@@ -66,6 +71,26 @@ __device__ __forceinline__ void widen(const Raw<TE, C>& r, float (&v)[C]) {
   for (int k = 0; k < C; ++k) {
     if constexpr (sizeof(TE) == 2) v[k] = k & 1 ? bf16_hi(r.w[k / 2]) : bf16_lo(r.w[k / 2]);
     else v[k] = __builtin_bit_cast(float, r.w[k]);
+  }
+}
+// C values of type TE through a descriptor: offsets outside its range store nothing.  No scalar offset on these: after a 16-byte buffer store
+// with an SGPR offset the compiler inserts no wait state, and here the next vector instruction overwrote the store's first data register
+// before it had been read.
+template <class TE, int C>
+__device__ __forceinline__ void bst(__amdgpu_buffer_rsrc_t r, unsigned off, const float (&v)[C]) {
+  if constexpr (sizeof(TE) == 2 && C == 8) {
+    const u32x4 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, 0);
+  } else if constexpr (sizeof(TE) == 2) {
+    const u32x2 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    __builtin_amdgcn_raw_buffer_store_b64(o, r, off, 0, 0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < C; k += 4) {
+      const u32x4 o = {__builtin_bit_cast(unsigned, v[k]), __builtin_bit_cast(unsigned, v[k + 1]), __builtin_bit_cast(unsigned, v[k + 2]),
+                       __builtin_bit_cast(unsigned, v[k + 3])};
+      __builtin_amdgcn_raw_buffer_store_b128(o, r, off + 4 * k, 0, 0);
+    }
   }
 }
 template <class TE, int C>
@@ -97,7 +122,7 @@ template <class TE, int C, int HLOG, int RW, bool SAVE, bool MX8>
 __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
   extern __shared__ float s_st[];                                       // [4][RW][dx] weighted V, [4][RW][H][2] maximum, sum
   const int n = a.n, dx = a.dx, H = a.H;
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
   const int NS = 64 >> a.lp_log, JS = 4 * NS;
   const bool act = li * C < dx;
   const int c = act ? li * C : 0, h = c / (C << HLOG);
@@ -119,78 +144,83 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
     bld(rq, act ? (t * dx + c) * 4 : OOB, rw.w);
     widen(rw, q[t]);
     const int i = min(i0 + t, n - 1);
-    mi[t] = nm[i] != 0;
+    mi[t] = __builtin_amdgcn_readfirstlane(t < rows ? (int)nm[i] : 0) != 0;
     gi[t] = grp ? grp[i] : 0;
     m[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
     for (int k = 0; k < C; ++k) { q[t][k] *= a.qscale; acc[t][k] = 0.f; }
   }
   const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
-  Raw<TE, C> e1n[RW], e2n[RW];
+  const __amdgpu_buffer_rsrc_t ry = rsrc((TE*)a.Y + row0 * n * dx, rows * n * dx * es);
+  const __amdgpu_buffer_rsrc_t rS = rsrc(SAVE ? a.S + row0 * n * H : nullptr, SAVE ? rows * n * H * 4 : 0);
+  const __amdgpu_buffer_rsrc_t rc = rsrc(MX8 ? a.q1 + row0 * n * dx : nullptr, MX8 ? rows * n * dx : 0);
+  const __amdgpu_buffer_rsrc_t rcs = rsrc(MX8 ? a.q1s + row0 * n * (dx / MX8_GROUP) : nullptr, MX8 ? rows * n * (dx / MX8_GROUP) : 0);
+  Raw<TE, C> e1n[RW], e2n[RW];          // a row's operands of the next key: loaded as soon as the present key's are widened
   Raw<float, C> kn, vn;
   // node flags of a key two steps ahead of its use: they decide the addresses of the next step's loads
   struct Meta { uint8_t m; int g; };
   auto meta = [&](int j) { const int jc = min(j, n - 1); return Meta{nm[jc], grp ? grp[jc] : 0}; };
-  auto fetch = [&](int j, Meta f) {
+  auto fetch_kv = [&](int j) {
     const unsigned ko = act && j < n ? (unsigned)(j * dx + c) * 4 : OOB;
     bld(rk, ko, kn.w); bld(rv, ko, vn.w);
-#pragma unroll
-    for (int t = 0; t < RW; ++t) {
-      const unsigned eo = act && j < n && f.m != 0 && mi[t] ? (unsigned)((t * n + j) * dx + c) * es : OOB;
-      bld(r1, eo, e1n[t].w); bld(r2, eo, e2n[t].w);
-    }
   };
+  // byte offset of a row's pair = the key's offset (one register for all rows) + the row's (uniform: the instruction's scalar offset); a row
+  // past the end, a masked pair, a key past the end: OOB.  E1 and E2 of masked pairs are not read
+  const unsigned row_c = (unsigned)(n * dx), row_e = row_c * es;
+  auto fetch = [&](int t, unsigned eo) {
+    const unsigned o = mi[t] ? eo : OOB, so = mi[t] ? t * row_e : 0;
+    bld(r1, o, e1n[t].w, so); bld(r2, o, e2n[t].w, so);
+  };
+  auto key_off = [&](int j, uint8_t mj) { return act & (j < n) & (mj != 0) ? (unsigned)(j * dx + c) * es : OOB; };
   const int jf = w * NS + slot;
   Meta f0 = meta(jf), f1 = meta(jf + JS);
-  fetch(jf, f0);
+  fetch_kv(jf);
+#pragma unroll
+  for (int t = 0; t < RW; ++t) fetch(t, key_off(jf, f0.m));
   for (int j0 = 0; j0 < n; j0 += JS) {
     const int j = j0 + jf;
-    Raw<TE, C> e1r[RW], e2r[RW];
     float kk[C], vv[C];
-#pragma unroll
-    for (int t = 0; t < RW; ++t) { e1r[t] = e1n[t]; e2r[t] = e2n[t]; }
     widen(kn, kk); widen(vn, vv);
     const int gj = j < n ? f0.g : -1;
     f0 = f1;
     f1 = meta(j + 2 * JS);
-    fetch(j + JS, f0);
+    fetch_kv(j + JS);
+    const bool st = act & (j < n);
+    const unsigned nx = key_off(j + JS, f0.m), jc = (unsigned)(j * dx + c), oY = st ? jc * es : OOB, oC = st ? jc : OOB;
+    const unsigned oS = st & ((li & ((1 << HLOG) - 1)) == 0) ? (unsigned)(j * H + h) * 4 : OOB;
+    const unsigned oCs = st & (c % MX8_GROUP == 0) ? (unsigned)(j * (dx / MX8_GROUP) + c / MX8_GROUP) : OOB;
 #pragma unroll
     for (int t = 0; t < RW; ++t) {
-      const bool st = j < n && t < rows;
-      const size_t pair = (row0 + t) * n + j;
       float e1[C], e2[C], y[C];
-      widen(e1r[t], e1); widen(e2r[t], e2);
+      widen(e1n[t], e1); widen(e2n[t], e2);
+      fetch(t, nx);
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < C; ++k) { y[k] = (q[t][k] * kk[k]) * (e1[k] + 1.f) + e2[k]; s += y[k]; }
-      if (st && act) gst((TE*)a.Y + pair * dx + c, y);
+      for (int k = 0; k < C; ++k) { const float x = q[t][k] * kk[k]; y[k] = fma_(x, e1[k], x + e2[k]); s += y[k]; }
+      bst<TE, C>(ry, oY + t * row_e, y);
       if constexpr (MX8) {
         unsigned mb = 0;
 #pragma unroll
         for (int k = 0; k < C; ++k) mb = dpp_max_u32(mb, abs_bits(e1[k]));
         const unsigned sb = mx8_scale(C == 8 ? quad_max(mb) : oct_max(mb));
         const float inv = mx8_inv(sb);
-        if (st && act) {
-          unsigned* d = reinterpret_cast<unsigned*>(a.q1 + pair * dx + c);
-          const unsigned w0 = mx8_pack4<false>(e1[0], e1[1], e1[2], e1[3], inv);
-          if constexpr (C == 8) *reinterpret_cast<uint2*>(d) = uint2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)};
-          else *d = w0;
-          if (c % MX8_GROUP == 0) a.q1s[pair * (dx / MX8_GROUP) + c / MX8_GROUP] = (uint8_t)sb;
-        }
+        const unsigned w0 = mx8_pack4<false>(e1[0], e1[1], e1[2], e1[3], inv), co = oC + t * row_c;
+        if constexpr (C == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)}, rc, co, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(w0, rc, co, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)sb, rcs, oCs + t * (row_c / MX8_GROUP), 0, 0);
       }
       s = head_sum<HLOG>(s);
       if (a.cap > 0.f) s = a.cap * tanhf(s * inv_cap);
       const bool on = gj >= 0 && gj == gi[t];
       s = on ? s : -INFINITY;
-      if constexpr (SAVE) {
-        if (st && act && (li & ((1 << HLOG) - 1)) == 0) a.S[pair * H + h] = s;
-      }
+      if constexpr (SAVE)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, s), rS, oS + t * (unsigned)(n * H) * 4, 0, 0);
       const float mx = fmaxf(m[t], s), mg = mx == -INFINITY ? 0.f : mx;
       const float sc = __expf(m[t] - mg), p = on ? __expf(s - mg) : 0.f;
       m[t] = mx;
-      l[t] = l[t] * sc + p;
+      l[t] = fma_(l[t], sc, p);
 #pragma unroll
-      for (int k = 0; k < C; ++k) acc[t][k] = acc[t][k] * sc + p * (on ? vv[k] : 0.f);
+      for (int k = 0; k < C; ++k) acc[t][k] = fma_(p, on ? vv[k] : 0.f, acc[t][k] * sc);
     }
   }
   for (int off = 1 << a.lp_log; off < 64; off <<= 1)                    // the key slots of the wave
@@ -198,10 +228,10 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
     for (int t = 0; t < RW; ++t) {
       const float mo = __shfl_xor(m[t], off), M = fmaxf(m[t], mo), mg = M == -INFINITY ? 0.f : M;
       const float x = __expf(m[t] - mg), y = __expf(mo - mg);
-      l[t] = l[t] * x + __shfl_xor(l[t], off) * y;
+      l[t] = fma_(l[t], x, __shfl_xor(l[t], off) * y);
       m[t] = M;
 #pragma unroll
-      for (int k = 0; k < C; ++k) acc[t][k] = acc[t][k] * x + __shfl_xor(acc[t][k], off) * y;
+      for (int k = 0; k < C; ++k) acc[t][k] = fma_(acc[t][k], x, __shfl_xor(acc[t][k], off) * y);
     }
   float* s_ml = s_st + 4 * RW * dx;
   if (slot == 0 && act) {
@@ -222,7 +252,7 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float x = __expf(s_ml[((k * RW + t) * H + hh) * 2] - mg);
-      L += s_ml[((k * RW + t) * H + hh) * 2 + 1] * x; A += s_st[(k * RW + t) * dx + cc] * x;
+      L = fma_(s_ml[((k * RW + t) * H + hh) * 2 + 1], x, L); A = fma_(s_st[(k * RW + t) * dx + cc], x, A);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;                         // no key: 0
     a.wV[(row0 + t) * dx + cc] = L == 0.f ? 0.f : A * inv;
@@ -235,18 +265,19 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
 // and dV_j are summed over the workgroup's rows in registers and LDS, and only one partial result per NW RW rows reaches memory.  dQ
 // stays in registers over the chunk.  k_attn_head_fold adds the partial results in order (no atomics: the sums do not depend on timing).
 #define HEAD_NW 8
-#define HEAD_RW 2
+// rows a wave: what its registers hold without spilling (two waves a SIMD)
+template <class TY> __host__ __device__ constexpr int head_rw() { return sizeof(TY) == 2 ? 4 : 2; }
 template <class TY, int C, int HLOG, bool MX8>
 __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
-  constexpr int RW = HEAD_RW, NW = HEAD_NW;
+  constexpr int RW = head_rw<TY>(), NW = HEAD_NW;
   extern __shared__ float s_kv[];                                       // [2][NW][NS][2][dx]
   const int n = a.n, dx = a.dx, H = a.H;
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
   const int NS = 64 >> a.lp_log;
   const bool act = li * C < dx;
   const int c = act ? li * C : 0, h = c / (C << HLOG);
   const int jc = blockIdx.x % a.njc, ib = (blockIdx.x / a.njc) % a.nib, b = blockIdx.x / a.njc / a.nib;
-  const int i0 = (ib * NW + w) * RW, rows = max(0, min(RW, n - i0));
+  const int i0 = (ib * NW + w) * RW, rows = __builtin_amdgcn_readfirstlane(max(0, min(RW, n - i0)));      // (uniform: descriptors are made of it)
   const int j_lo = jc * a.jchunk, j_hi = min(n, j_lo + a.jchunk);
   const size_t node0 = (size_t)b * n, row0 = node0 + min(i0, n - 1);
   const uint8_t* nm = a.nm + node0;
@@ -254,6 +285,7 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
   const __amdgpu_buffer_rsrc_t r1 = MX8 ? rsrc((const uint8_t*)a.E1 + row0 * n * dx, range) : rsrc((const TY*)a.E1 + row0 * n * dx, range * es);
   const __amdgpu_buffer_rsrc_t rsc = rsrc(MX8 ? a.E1s + row0 * n * (dx / MX8_GROUP) : nullptr, MX8 ? range / MX8_GROUP : 0);
   const __amdgpu_buffer_rsrc_t ry = rsrc((const TY*)a.dY + row0 * n * dx, range * es);
+  const __amdgpu_buffer_rsrc_t r1o = rsrc((TY*)a.dE1 + row0 * n * dx, range * es), r2o = rsrc((TY*)a.dE2 + row0 * n * dx, range * es);
   const __amdgpu_buffer_rsrc_t rS = rsrc(a.S + row0 * n * H, rows * n * H * 4);
   const __amdgpu_buffer_rsrc_t rk = rsrc(a.K + node0 * dx, n * dx * 4), rv = rsrc(a.V + node0 * dx, n * dx * 4);
   const __amdgpu_buffer_rsrc_t rq = rsrc(a.Q + row0 * dx, rows * dx * 4), ro = rsrc(a.wV + row0 * dx, rows * dx * 4), rg = rsrc(a.dwV + row0 * dx, rows * dx * 4);
@@ -268,88 +300,100 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
     float o[C], d = 0.f;
     bld(ro, off, x.w); widen(x, o);
 #pragma unroll
-    for (int k = 0; k < C; ++k) { d += g[t][k] * o[k]; q[t][k] *= a.qscale; dq[t][k] = 0.f; }
+    for (int k = 0; k < C; ++k) { d = fma_(g[t][k], o[k], d); q[t][k] *= a.qscale; dq[t][k] = 0.f; }
     D[t] = head_sum<HLOG>(d);
     const int i = min(i0 + t, n - 1);
-    mi[t] = t < rows && nm[i] != 0;
+    mi[t] = __builtin_amdgcn_readfirstlane(t < rows ? (int)nm[i] : 0) != 0;
     const float2 st = *reinterpret_cast<const float2*>(a.stat + ((node0 + i) * H + h) * 2);
     mx[t] = t < rows ? st.x : 0.f; il[t] = t < rows ? st.y : 0.f;
   }
   const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
   constexpr int W1 = MX8 ? C / 4 : (int)sizeof(TY) * C / 4;
   struct Ops { unsigned e1[W1], sc, s; Raw<TY, C> dy; };
-  Ops nx[RW];
+  Ops op[RW];                           // a row's operands of the next key: loaded as soon as the present key's are widened
   Raw<float, C> kn, vn;
   auto meta = [&](int j) { return nm[min(j, n - 1)]; };
-  auto fetch = [&](int j, uint8_t mj) {
-    const bool on = act && j < j_hi;
-    const unsigned ko = on ? (unsigned)(j * dx + c) * 4 : OOB;
+  auto fetch_kv = [&](int j) {
+    const unsigned ko = act && j < j_hi ? (unsigned)(j * dx + c) * 4 : OOB;
     bld(rk, ko, kn.w); bld(rv, ko, vn.w);
-#pragma unroll
-    for (int t = 0; t < RW; ++t) {
-      const unsigned p = (unsigned)(t * n + j), e = p * dx + c;
-      const bool pm = on && mj != 0 && mi[t];
-      bld(r1, pm ? (MX8 ? e : e * es) : OOB, nx[t].e1);
-      if constexpr (MX8) nx[t].sc = __builtin_amdgcn_raw_buffer_load_b8(rsc, pm ? p * (dx / MX8_GROUP) + c / MX8_GROUP : OOB, 0, 0);
-      bld(ry, on ? e * es : OOB, nx[t].dy.w);
-      nx[t].s = __builtin_amdgcn_raw_buffer_load_b32(rS, on ? (p * H + h) * 4 : OOB, 0, 0);
-    }
+  };
+  // (offsets as in the forward: the key's in one register for all rows, the row's uniform)
+  struct Off { unsigned e1, sc, y, s; };
+  auto key_off = [&](int j, uint8_t mj) {
+    const bool on = act & (j < j_hi), pm = on & (mj != 0);
+    const unsigned jc = (unsigned)(j * dx + c);
+    return Off{pm ? (MX8 ? jc : jc * es) : OOB, pm ? (unsigned)(j * (dx / MX8_GROUP) + c / MX8_GROUP) : OOB, on ? jc * es : OOB,
+               on ? (unsigned)(j * H + h) * 4 : OOB};
+  };
+  const unsigned row_c = (unsigned)(n * dx), row_e = row_c * es;
+  auto fetch = [&](int t, const Off& o) {
+    const bool in = t < rows;
+    bld(r1, mi[t] ? o.e1 : OOB, op[t].e1, mi[t] ? t * (MX8 ? row_c : row_e) : 0);
+    if constexpr (MX8) op[t].sc = __builtin_amdgcn_raw_buffer_load_b8(rsc, mi[t] ? o.sc : OOB, mi[t] ? t * (row_c / MX8_GROUP) : 0, 0);
+    bld(ry, in ? o.y : OOB, op[t].dy.w, in ? t * row_e : 0);
+    op[t].s = __builtin_amdgcn_raw_buffer_load_b32(rS, in ? o.s : OOB, in ? (unsigned)(t * n * H) * 4 : 0, 0);
   };
   uint8_t m0 = meta(j_lo + slot), m1 = meta(j_lo + slot + NS);
-  fetch(j_lo + slot, m0);
+  fetch_kv(j_lo + slot);
+#pragma unroll
+  for (int t = 0; t < RW; ++t) fetch(t, key_off(j_lo + slot, m0));
+  // what this thread adds up of the waves' dK_j, dV_j: one quad of one key slot (NS 2 dx / 4 <= 256 of them)
+  const int quads = 2 * dx / 4, r_sl = threadIdx.x / quads, r_c = (threadIdx.x - r_sl * quads) * 4, r_src = r_sl * 2 * dx + r_c;
+  const bool red = r_sl < NS, red_k = r_c < dx;
+  const size_t part0 = (((size_t)ib * a.B + b) * n + j_lo) * dx;
+  const __amdgpu_buffer_rsrc_t rdk = rsrc(a.dKp + part0, (j_hi - j_lo) * dx * 4), rdv = rsrc(a.dVp + part0, (j_hi - j_lo) * dx * 4);
+  unsigned r_off = (unsigned)(r_sl * dx + (red_k ? r_c : r_c - dx)) * 4;
   int buf = 0;
   for (int j0 = j_lo; j0 < j_hi; j0 += NS, buf ^= 1) {
     const int j = j0 + slot;
-    Ops cu[RW];
     float kk[C], vv[C], dk[C], dv[C];
-#pragma unroll
-    for (int t = 0; t < RW; ++t) cu[t] = nx[t];
     widen(kn, kk); widen(vn, vv);
-    const bool mj = j < j_hi && m0 != 0;
+    const bool mj = (j < j_hi) & (m0 != 0);
     m0 = m1;
     m1 = meta(j + 2 * NS);
-    fetch(j + NS, m0);
+    fetch_kv(j + NS);
+    const Off nx = key_off(j + NS, m0);
+    const unsigned oE = act & (j < j_hi) ? (unsigned)(j * dx + c) * es : OOB;
 #pragma unroll
     for (int k = 0; k < C; ++k) dk[k] = dv[k] = 0.f;
 #pragma unroll
     for (int t = 0; t < RW; ++t) {
       float e1[C], G[C], o1[C], o2[C], dp = 0.f;
       if constexpr (MX8) {
-        const float step = mx8_step(cu[t].sc < MX8_B_MIN ? MX8_B_MIN : cu[t].sc);          // (a masked pair reads 0)
+        const float step = mx8_step(op[t].sc < MX8_B_MIN ? MX8_B_MIN : op[t].sc);          // (a masked pair reads 0)
 #pragma unroll
         for (int k = 0; k < C; k += 4) {
-          e1[k] = mx8_elem<0>(cu[t].e1[k / 4]) * step; e1[k + 1] = mx8_elem<1>(cu[t].e1[k / 4]) * step;
-          e1[k + 2] = mx8_elem<2>(cu[t].e1[k / 4]) * step; e1[k + 3] = mx8_elem<3>(cu[t].e1[k / 4]) * step;
+          e1[k] = mx8_elem<0>(op[t].e1[k / 4]) * step; e1[k + 1] = mx8_elem<1>(op[t].e1[k / 4]) * step;
+          e1[k + 2] = mx8_elem<2>(op[t].e1[k / 4]) * step; e1[k + 3] = mx8_elem<3>(op[t].e1[k / 4]) * step;
         }
       } else {
         Raw<TY, C> r;
 #pragma unroll
-        for (int k = 0; k < W1; ++k) r.w[k] = cu[t].e1[k];
+        for (int k = 0; k < W1; ++k) r.w[k] = op[t].e1[k];
         widen(r, e1);
       }
-      widen(cu[t].dy, G);
+      widen(op[t].dy, G);
+      const float s = __builtin_bit_cast(float, op[t].s), cs = s * inv_cap;
+      fetch(t, nx);
 #pragma unroll
-      for (int k = 0; k < C; ++k) dp += g[t][k] * vv[k];
+      for (int k = 0; k < C; ++k) dp = fma_(g[t][k], vv[k], dp);
       dp = head_sum<HLOG>(dp);
-      const float s = __builtin_bit_cast(float, cu[t].s), cs = s * inv_cap;
-      const bool on = t < rows && j < j_hi && s != -INFINITY;
+      const bool on = (t < rows) & (j < j_hi) & (s != -INFINITY);
       const float p = on ? __expf(s - mx[t]) * il[t] : 0.f;
-      const float ds = on ? p * (dp - D[t]) * (1.f - cs * cs) : 0.f;
-      const bool pm = mj && mi[t];
+      const float ds = on ? p * (dp - D[t]) * fma_(-cs, cs, 1.f) : 0.f;
+      const bool pm = mj & mi[t];
 #pragma unroll
       for (int k = 0; k < C; ++k) {
         G[k] += ds;
         o2[k] = pm ? G[k] : 0.f;
         o1[k] = o2[k] * (q[t][k] * kk[k]);
-        const float x = G[k] * (e1[k] + 1.f);
-        dq[t][k] += x * kk[k];
-        dk[k] += x * q[t][k];
-        dv[k] += p * g[t][k];
+        const float x = fma_(G[k], e1[k], G[k]);
+        dq[t][k] = fma_(x, kk[k], dq[t][k]);
+        dk[k] = fma_(x, q[t][k], dk[k]);
+        dv[k] = fma_(p, g[t][k], dv[k]);
       }
-      if (t < rows && j < j_hi && act) {
-        const size_t e = ((row0 + t) * n + j) * dx + c;
-        gst((TY*)a.dE1 + e, o1); gst((TY*)a.dE2 + e, o2);
-      }
+      bst<TY, C>(r1o, oE + t * row_e, o1); bst<TY, C>(r2o, oE + t * row_e, o2);
+      __builtin_amdgcn_sched_barrier(0);                                // one row's temporaries at a time: mixed, the rows spill
     }
     float* mine = s_kv + (((buf * NW + w) * NS + slot) * 2) * dx + c;
     if (act) { gst(mine, dk); gst(mine + dx, dv); }
@@ -357,19 +401,18 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     // the waves' sums; the other buffer is written next, and this one again only after the barrier that follows this read
-    const int quads = 2 * dx / 4;
-    for (int u = threadIdx.x; u < NS * quads; u += 64 * NW) {
-      const int sl = u / quads, cq = u - sl * quads;
-      const float* src = s_kv + ((buf * NW * NS + sl) * 2) * dx + cq * 4;
+    if (red) {
+      const float* src = s_kv + (size_t)buf * NW * NS * 2 * dx + r_src;
       float4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
-        const float4 x = *reinterpret_cast<const float4*>(src + (size_t)k * NS * 2 * dx);
+        const float4 x = *reinterpret_cast<const float4*>(src + k * NS * 2 * dx);
         t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
       }
-      const int cc = cq * 4 < dx ? cq * 4 : cq * 4 - dx;
-      float* dst = (cq * 4 < dx ? a.dKp : a.dVp) + (((size_t)ib * a.B + b) * n + j0 + sl) * dx + cc;
-      if (j0 + sl < j_hi) *reinterpret_cast<float4*>(dst) = t;
+      const u32x4 o = __builtin_bit_cast(u32x4, t);
+      __builtin_amdgcn_raw_buffer_store_b128(o, rdk, red_k ? r_off : OOB, 0, 0);         // (keys past the chunk are outside the range)
+      __builtin_amdgcn_raw_buffer_store_b128(o, rdv, red_k ? OOB : r_off, 0, 0);
+      r_off += (unsigned)(NS * dx) * 4;
     }
   }
   for (int off = 1 << a.lp_log; off < 64; off <<= 1)
@@ -418,18 +461,18 @@ static bool head_shape(int dx, int H, int* C, int* hlog, int* lp_log) {
   *lp_log = p;
   return true;
 }
-// backward: the row blocks and the keys' chunks: enough workgroups to fill the chip (2 per CU), chunks of at least 8 steps
-static void head_chunks(int B, int n, int lp_log, int* nib, int* njc, int* jchunk) {
-  const int NS = 64 >> lp_log;
-  *nib = (n + HEAD_NW * HEAD_RW - 1) / (HEAD_NW * HEAD_RW);
-  const long long have = (long long)B * *nib;
-  int want = (int)((512 + have - 1) / have);
-  const int most = (n + 8 * NS - 1) / (8 * NS);
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  *jchunk = (n + want - 1) / want;
-  *jchunk = (*jchunk + NS - 1) / NS * NS;
-  *njc = (n + *jchunk - 1) / *jchunk;
+// backward: row blocks, and the keys cut into chunks so that the workgroups fill the 256 CUs in whole rounds.  One workgroup runs on a CU at a
+// time (its registers); it takes its chunk's steps and HEAD_FIXED more for its beginning and end.
+#define HEAD_FIXED 6
+static void head_chunks(int B, int n, int lp_log, bool bf16, int* nib, int* njc, int* jchunk) {
+  const int NS = 64 >> lp_log, rows = HEAD_NW * (bf16 ? head_rw<bf16_t>() : head_rw<float>());
+  *nib = (n + rows - 1) / rows;
+  long long best = -1;
+  for (int want = 1; want <= 64 && (want == 1 || (want - 1) * 4 * NS < n); ++want) {
+    const int ch = ((n + want - 1) / want + NS - 1) / NS * NS, nc = (n + ch - 1) / ch;
+    const long long rounds = ((long long)B * *nib * nc + 255) / 256, cost = rounds * (ch / NS + HEAD_FIXED);
+    if (best < 0 || cost < best) { best = cost; *jchunk = ch; *njc = nc; }
+  }
 }
 
 template <class TE, int C, int HLOG>
@@ -503,11 +546,11 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
   return DA_OK;
 }
 
-long long da_attn_head_bwd_workspace(int B, int n, int dx, int n_head) {
+long long da_attn_head_bwd_workspace(int B, int n, int dx, int n_head, int dy_bf16) {
   int C, hlog, lp, nib, njc, jchunk;
   if (B < 0 || n < 0 || !head_shape(dx, n_head, &C, &hlog, &lp)) return -1;
   if (B == 0 || n == 0) return 0;
-  head_chunks(B, n, lp, &nib, &njc, &jchunk);
+  head_chunks(B, n, lp, dy_bf16 != 0, &nib, &njc, &jchunk);
   return (long long)sizeof(float) * ((nib > 1 ? 2LL * nib : 0) + (njc > 1 ? njc : 0)) * B * n * dx;
 }
 
@@ -526,11 +569,11 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
   DA_CHECK_ARG(cap >= 0.f && cap < INFINITY, "da_attn_head_bwd: cap = %g", cap);
   DA_CHECK_ARG(al16({Q, K, V, E1, E1_codes, wV, dY, dwV, dQ, dK, dV, dE1, dE2, workspace}) && ((uintptr_t)stat & 7) == 0 && ((uintptr_t)S & 3) == 0,
                "da_attn_head_bwd: unaligned tensor (16 bytes)");
-  const long long need = da_attn_head_bwd_workspace(B, n, dx, n_head);
+  const long long need = da_attn_head_bwd_workspace(B, n, dx, n_head, dy_bf16);
   DA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "da_attn_head_bwd: workspace too small");
   a.Q = Q; a.K = K; a.V = V; a.E1 = E1_codes ? E1_codes : E1; a.E1s = E1_scales; a.nm = node_mask; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx;
   a.H = n_head; a.wV = (float*)wV; a.S = (float*)S; a.stat = (float*)stat; a.dY = dY; a.dwV = dwV; a.dE1 = dE1; a.dE2 = dE2; a.B = B;
-  head_chunks(B, n, a.lp_log, &a.nib, &a.njc, &a.jchunk);
+  head_chunks(B, n, a.lp_log, dy_bf16 != 0, &a.nib, &a.njc, &a.jchunk);
   const size_t one = (size_t)B * n * dx;
   float* ws = (float*)workspace;
   a.dKp = dK; a.dVp = dV; a.dQp = dQ;

@@ -66,8 +66,8 @@ def test_c_entries_refuse_before_any_launch():
     bwd = lambda **k: lib.da_attn_head_bwd(*[{**dict(Q=p, K=p, V=p, E1=p, c=0, sc=0, nm=p, qs=1.0, cap=0.0, wV=p, S=p, st=p, dY=p, bf=0, g=p, dQ=p, dK=p, dV=p, d1=p,
                                                       d2=p, ws=p, nb=0, B=1, n=300, dx=64, H=4, s=0), **k}[x] for x in ('Q', 'K', 'V', 'E1', 'c', 'sc', 'nm', 'qs', 'cap',
                                               'wV', 'S', 'st', 'dY', 'bf', 'g', 'dQ', 'dK', 'dV', 'd1', 'd2', 'ws', 'nb', 'B', 'n', 'dx', 'H', 's')])
-    assert lib.da_attn_head_bwd_workspace(1, 300, 64, 4) > 0 and lib.da_attn_head_bwd_workspace(1, 1, 64, 4) == 0
-    assert lib.da_attn_head_bwd_workspace(1, 300, 64, 5) == -1 and lib.da_attn_head_bwd_workspace(0, 300, 64, 4) == 0
+    assert lib.da_attn_head_bwd_workspace(1, 300, 64, 4, 0) > 0 and lib.da_attn_head_bwd_workspace(1, 1, 64, 4, 0) == 0
+    assert lib.da_attn_head_bwd_workspace(1, 300, 64, 5, 0) == -1 and lib.da_attn_head_bwd_workspace(0, 300, 64, 4, 0) == 0
     assert bwd() == -1 and b'workspace' in lib.da_last_error()
     assert bwd(E1=0) == -1 and bwd(c=p, sc=p) == -1 and bwd(E1=0, c=p) == -1 and bwd(dY=0) == -1 and bwd(H=5) == -3 and bwd(B=0) == 0
     assert bwd(dQ=8) == -1 and b'unaligned' in lib.da_last_error()
