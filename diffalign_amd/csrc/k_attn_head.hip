@@ -47,20 +47,24 @@ struct HeadArgs {
 };
 
 #define OOB 0x80000000u                 // past every descriptor's range, also with a row's offset added (the host keeps both below 2^31)
+// cache policy of the streams that pass once (E1, E2, Y, dY, dE1, dE2): non-temporal for bf16, so that K and V keep the L2 (forward B = 16,
+// n = 140 96 -> 88 us, backward n = 300 565 -> 532 us); fp32 takes two instructions for a lane's 8 channels, each touching half of
+// every 64 bytes, and wants the line kept for the second (forward / backward n = 93 49 / 49 us, non-temporal 52 / 55)
+template <class TE> constexpr int nt() { return sizeof(TE) == 2 ? 2 : 0; }
 template <class TE, int C> struct Raw { unsigned w[sizeof(TE) * C / 4]; };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, unsigned bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
 }
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
-template <int W>
+template <int AUX = 0, int W>
 __device__ __forceinline__ void bld(__amdgpu_buffer_rsrc_t r, unsigned off, unsigned (&w)[W], unsigned soff = 0) {
-  if constexpr (W == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0);
-  else if constexpr (W == 2) { const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0); w[0] = v.x; w[1] = v.y; }
+  if constexpr (W == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, AUX);
+  else if constexpr (W == 2) { const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, AUX); w[0] = v.x; w[1] = v.y; }
   else {
 #pragma unroll
     for (int k = 0; k < W / 4; ++k) {
-      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, soff, 0);
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, soff, AUX);
       w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
     }
   }
@@ -80,16 +84,16 @@ template <class TE, int C>
 __device__ __forceinline__ void bst(__amdgpu_buffer_rsrc_t r, unsigned off, const float (&v)[C]) {
   if constexpr (sizeof(TE) == 2 && C == 8) {
     const u32x4 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
-    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, nt<TE>());
   } else if constexpr (sizeof(TE) == 2) {
     const u32x2 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-    __builtin_amdgcn_raw_buffer_store_b64(o, r, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b64(o, r, off, 0, nt<TE>());
   } else {
 #pragma unroll
     for (int k = 0; k < C; k += 4) {
       const u32x4 o = {__builtin_bit_cast(unsigned, v[k]), __builtin_bit_cast(unsigned, v[k + 1]), __builtin_bit_cast(unsigned, v[k + 2]),
                        __builtin_bit_cast(unsigned, v[k + 3])};
-      __builtin_amdgcn_raw_buffer_store_b128(o, r, off + 4 * k, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(o, r, off + 4 * k, 0, nt<TE>());
     }
   }
 }
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
   const unsigned row_c = (unsigned)(n * dx), row_e = row_c * es;
   auto fetch = [&](int t, unsigned eo) {
     const unsigned o = mi[t] ? eo : OOB, so = mi[t] ? t * row_e : 0;
-    bld(r1, o, e1n[t].w, so); bld(r2, o, e2n[t].w, so);
+    bld<nt<TE>()>(r1, o, e1n[t].w, so); bld<nt<TE>()>(r2, o, e2n[t].w, so);
   };
   auto key_off = [&](int j, uint8_t mj) { return act & (j < n) & (mj != 0) ? (unsigned)(j * dx + c) * es : OOB; };
   const int jf = w * NS + slot;
@@ -205,8 +209,8 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
         const unsigned sb = mx8_scale(C == 8 ? quad_max(mb) : oct_max(mb));
         const float inv = mx8_inv(sb);
         const unsigned w0 = mx8_pack4<false>(e1[0], e1[1], e1[2], e1[3], inv), co = oC + t * row_c;
-        if constexpr (C == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)}, rc, co, 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b32(w0, rc, co, 0, 0);
+        if constexpr (C == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)}, rc, co, 0, nt<TE>());
+        else __builtin_amdgcn_raw_buffer_store_b32(w0, rc, co, 0, nt<TE>());
         __builtin_amdgcn_raw_buffer_store_b8((uint8_t)sb, rcs, oCs + t * (row_c / MX8_GROUP), 0, 0);
       }
       s = head_sum<HLOG>(s);
@@ -328,9 +332,9 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
   const unsigned row_c = (unsigned)(n * dx), row_e = row_c * es;
   auto fetch = [&](int t, const Off& o) {
     const bool in = t < rows;
-    bld(r1, mi[t] ? o.e1 : OOB, op[t].e1, mi[t] ? t * (MX8 ? row_c : row_e) : 0);
+    bld<nt<TY>()>(r1, mi[t] ? o.e1 : OOB, op[t].e1, mi[t] ? t * (MX8 ? row_c : row_e) : 0);
     if constexpr (MX8) op[t].sc = __builtin_amdgcn_raw_buffer_load_b8(rsc, mi[t] ? o.sc : OOB, mi[t] ? t * (row_c / MX8_GROUP) : 0, 0);
-    bld(ry, in ? o.y : OOB, op[t].dy.w, in ? t * row_e : 0);
+    bld<nt<TY>()>(ry, in ? o.y : OOB, op[t].dy.w, in ? t * row_e : 0);
     op[t].s = __builtin_amdgcn_raw_buffer_load_b32(rS, in ? o.s : OOB, in ? (unsigned)(t * n * H) * 4 : 0, 0);
   };
   uint8_t m0 = meta(j_lo + slot), m1 = meta(j_lo + slot + NS);
@@ -439,9 +443,13 @@ __global__ void __launch_bounds__(256) k_attn_head_fold(const float4* __restrict
   const float4* src = which == 0 ? pQ : which == 1 ? pK : pV;
   const int G = which == 0 ? njc : nib;
   float4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int g = 0; g < G; ++g) {
-    const float4 x = src[(size_t)g * quads + t];
-    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  for (int g = 0; g < G; g += 5) {                                        // five in flight, added in order
+    float4 x[5];
+#pragma unroll
+    for (int u = 0; u < 5; ++u) x[u] = src[(size_t)min(g + u, G - 1) * quads + t];
+#pragma unroll
+    for (int u = 0; u < 5; ++u)
+      if (g + u < G) { s.x += x[u].x; s.y += x[u].y; s.z += x[u].z; s.w += x[u].w; }
   }
   (which == 0 ? dQ : which == 1 ? dK : dV)[t] = s;
 }
@@ -477,7 +485,9 @@ static void head_chunks(int B, int n, int lp_log, bool bf16, int* nib, int* njc,
 
 template <class TE, int C, int HLOG>
 static void fwd_launch(const HeadArgs& a, bool save, bool mx8, hipStream_t s) {
-  constexpr int WIDE = sizeof(TE) == 2 ? 4 : 2;                         // rows per workgroup where that still gives 2 workgroups per CU, else 1
+  // rows per workgroup: 2 share K_j and V_j (3 and 4 take registers that are waves: 194 against 199 and 213 us, 1 row 226 us, bf16 B = 8, n = 300)
+  // where that still gives 2 workgroups per CU, else 1
+  constexpr int WIDE = 2;
   const bool wide = (long long)a.B * ((a.n + WIDE - 1) / WIDE) >= 512;
   const int RW = wide ? WIDE : 1;
   const long long grid = (long long)a.B * ((a.n + RW - 1) / RW);

@@ -125,9 +125,10 @@ struct WgradCfg {
   static constexpr int WT = TILES < 4 ? TILES : 4, WK = 4 / WT;         // waves over result tiles x waves over rows
   static constexpr int WO = TO >= WT ? WT : (TO >= 2 && WT == 4 ? 2 : TO), WI = WT / WO;
   static constexpr int AO = TO / WO, AI = TI / WI;                      // tiles per wave
-  static constexpr int KR = WK == 4 ? 64 : 32, KSTEPS = KR / 16;        // rows per LDS tile
   static constexpr int PLANES = sizeof(TY) == 4 ? 3 : 1;
   static constexpr int PY = tr_pitch(OUT), PX = tr_pitch(IN);
+  // rows per LDS tile: 64 where two workgroups still fit a CU (fp32 64 -> 256 does not: 131 KB)
+  static constexpr int KR = 64 * (PLANES * PY + PX) + 8192 <= 80 * 1024 ? 64 : 32, KSTEPS = KR / 16;
   static constexpr int Y_BYTES = KR * PY, X_BYTES = KR * PX;
   static constexpr int NYT = KR * OUT / 8;                              // chunks of 8 features in a tile
   static constexpr int NXT = KR * IN / 8;
@@ -290,10 +291,12 @@ __global__ void __launch_bounds__(256) k_mx8_wgrad_fold(const float4* __restrict
   }
 }
 
-#define MX8_WGRAD_SLICES 512
-static long long wgrad_slice_rows(long long R, int KR) {
-  long long per = (R + MX8_WGRAD_SLICES - 1) / MX8_WGRAD_SLICES;
-  return (per + KR - 1) / KR * KR;
+// Rows of a slice, a multiple of 64.  Up to 131,072 rows 256 slices (one workgroup a CU), beyond that 512: the second workgroup hides the
+// first one's waits, and its partial result costs the fold.  256 / 512 slices, kernel and fold: 64 -> 256 bf16 60,000 rows 18 / 21 us,
+// 313,600 rows 42 / 40 us; 128 -> 64 14 / 18 us, 28 / 25 us.
+static long long wgrad_slice_rows(long long R) {
+  const long long G = R <= 131072 ? 256 : 512, per = (R + G - 1) / G;
+  return (per + 63) / 64 * 64;
 }
 static int wgrad_wk(int in_features, int out_features) { const int tiles = in_features * out_features / 1024; return tiles < 4 ? 4 / tiles : 1; }
 static bool wgrad_built(int i, int o) {
@@ -303,7 +306,7 @@ static bool wgrad_built(int i, int o) {
 template <int IN, int OUT, class TY>
 static void launch_mx8_wgrad(const uint8_t* codes, const uint8_t* scales, const TY* dY, float* dW, float* db, float* ws, long long R, hipStream_t s) {
   using C = WgradCfg<IN, OUT, TY>;
-  const long long per = wgrad_slice_rows(R, C::KR);
+  const long long per = wgrad_slice_rows(R);
   const int G = (int)((R + per - 1) / per);
   float* bpart = ws + (size_t)G * C::WK * OUT * IN;
   k_mx8_wgrad<IN, OUT, TY><<<G, 256, 0, s>>>(codes, scales, dY, ws, bpart, R, (int)per);
@@ -396,7 +399,7 @@ int da_relu_dropout_bwd_mx8(const void* codes, const void* dy, void* dx, int is_
 long long da_linear_wgrad_mx8_workspace(long long R, int in_features, int out_features) {
   if (R < 0 || !wgrad_built(in_features, out_features)) return -1;
   const int wk = wgrad_wk(in_features, out_features);
-  const long long per = R ? wgrad_slice_rows(R, wk == 4 ? 64 : 32) : 1, G = (R + per - 1) / per;
+  const long long per = R ? wgrad_slice_rows(R) : 1, G = (R + per - 1) / per;
   return (long long)sizeof(float) * G * ((long long)wk * in_features * out_features + out_features);
 }
 int da_linear_wgrad_mx8(const void* codes, const uint8_t* scales, const void* dY, int dy_bf16, float* dW, float* db, void* workspace,

@@ -2,7 +2,7 @@
 
 Tolerances.  Codes, scales and restored values: equal, bit for bit.  Weight gradient: every product of an 8-bit x and a bf16 dY (or a
 third of an fp32 dY; what the three parts leave of it is below 2^-26 relative) is exact in fp32, so only the fp32 sums round: a slice
-adds at most 64 rows here (R <= 512 * 64), the fold at most 32 + 16 partial results; each addition is off by at most 2^-23 of the
+adds at most 64 rows here (R <= 256 * 64), the fold at most 32 + 16 partial results; each addition is off by at most 2^-23 of the
 running magnitude (the matrix unit may truncate instead of rounding), which is at most S = sum |dY| |x|: 112 * 2^-23 S.
 Column sums likewise, with S = sum |dY|."""
 import pytest
@@ -114,14 +114,14 @@ def test_linear_wgrad(shape, dtype):
 
 
 def test_linear_wgrad_many_rows_and_nonfinite():
-    """More rows than 512 slices of one tile; an infinite and a NaN gradient reach exactly their own row of dW and element of db."""
+    """Slices of several tiles; an infinite and a NaN gradient reach exactly their own row of dW and element of db."""
     from diffalign_amd import mx8
     R, i, o = 70_001, 64, 64
     codes, scales, x = Q.quantize(act(R, i, torch.float32, 1))
     dy = act(R, o, torch.float32, 2)
     dW, db = mx8.linear_wgrad(mx8.Mx8(codes.to(D_), scales.to(D_)), dy.to(D_))
     S = dy.double().abs().t() @ x.abs()
-    assert ((dW.cpu().double() - dy.double().t() @ x).abs() <= (160 + 48) * 2.0 ** -23 * S).all()      # slices of 160 rows
+    assert ((dW.cpu().double() - dy.double().t() @ x).abs() <= (320 + 48) * 2.0 ** -23 * S).all()      # slices of 320 rows
     dy[40_000, 3], dy[5, 7] = float('inf'), float('nan')
     dW, db = mx8.linear_wgrad(mx8.Mx8(codes.to(D_), scales.to(D_)), dy.to(D_))
     ok = torch.ones(o, dtype=torch.bool); ok[3] = ok[7] = False
