@@ -5,6 +5,7 @@ differentiated by autograd itself).  fp32 throughout."""
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 from torch.autograd import Function
@@ -111,6 +112,64 @@ class WideLinearBF16(Function):
         return dx, dW, db, None
 
 
+class WideLinearMx8(Function):
+    """nn.Linear over the pairs whose input is held in 8 bits for the backward (mx8.py), fp32 or bf16: the forward uses x itself, dW / db come
+    from da_linear_wgrad_mx8 on the 8-bit x, dX is a library GEMM as in the other two.  codes, scales: the caller's 8-bit form of x (the two
+    Linears of one input share it)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, codes, scales):
+        w, b = (weight, bias) if x.dtype == torch.float32 else (weight.to(x.dtype), bias.to(x.dtype))
+        ctx.save_for_backward(codes, scales, w)
+        return torch.nn.functional.linear(x, w, b)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scales, w = ctx.saved_tensors
+        dy = dy.contiguous()
+        dW, db = mx8.linear_wgrad(mx8.Mx8(codes, scales), dy)
+        return (dy @ w if ctx.needs_input_grad[0] else None), dW, db, None, None
+
+
+class FeedForwardMx8(Function):
+    """lin2(dropout_p(relu(lin1(x)))) over the pairs (layers.py:353-357) with both Linears' inputs held in 8 bits.  The hidden tensor is
+    quantised so that what is not zero stays so: its codes are the ReLU's and the dropout's mask as well."""
+
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, seed, salt, p):
+        q = mx8.quantize(x)
+        if x.dtype != torch.float32:
+            w1, b1, w2, b2 = (t.to(x.dtype) for t in (w1, b1, w2, b2))
+        h = _relu_dropout_(torch.nn.functional.linear(x, w1, b1), seed, salt, p)
+        qh = mx8.quantize(h, keep_nonzero=True)
+        ctx.save_for_backward(*q, *qh, w1, w2)
+        ctx.p = float(p)
+        return torch.nn.functional.linear(h, w2, b2)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scales, hc, hs, w1, w2 = ctx.saved_tensors
+        dy = dy.contiguous()
+        dW2, db2 = mx8.linear_wgrad(mx8.Mx8(hc, hs), dy)
+        dh = mx8.relu_dropout_bwd(mx8.Mx8(hc, hs), dy @ w2, ctx.p)
+        dW1, db1 = mx8.linear_wgrad(mx8.Mx8(codes, scales), dh)
+        return (dh @ w1 if ctx.needs_input_grad[0] else None), dW1, db1, dW2, db2, None, None, None
+
+
+def _mx8_linear(lin: torch.nn.Linear) -> bool:
+    return (lin.in_features, lin.out_features) in mx8.WGRAD_SHAPES and lin.bias is not None and torch.is_grad_enabled()
+
+
+def feed_forward(lin1: torch.nn.Linear, lin2: torch.nn.Linear, x: torch.Tensor, act, checkpoint: str = 'none') -> torch.Tensor:
+    """lin2(dropout_p(relu(lin1(x)))) per pair, act = (seed, salt, p); checkpoint='mx8' (where both Linears are built for it): the backward
+    gets x and the hidden tensor in 8 bits."""
+    if checkpoint == 'mx8' and _mx8_linear(lin1) and _mx8_linear(lin2):
+        return FeedForwardMx8.apply(x, lin1.weight, lin1.bias, lin2.weight, lin2.bias, *act)
+    return wide_linear(lin2, wide_linear(lin1, x, act=act))
+
+
 def _relu_dropout_(h, seed, salt, p):
     p = float(p)
     L.check(L.lib().da_relu_dropout(L.ptr(h), int(h.dtype == torch.bfloat16), h.numel(), L.ptr(seed if p > 0 else None), salt, p, L.stream()),
@@ -128,11 +187,14 @@ def _relu_dropout_bwd(h, dy, p):
     return dx
 
 
-def wide_linear(lin: torch.nn.Linear, x: torch.Tensor, act=None) -> torch.Tensor:
+def wide_linear(lin: torch.nn.Linear, x: torch.Tensor, act=None, held: Optional[mx8.Mx8] = None) -> torch.Tensor:
     """`lin(x)` for per-pair inputs: WideLinear where da_linear_wgrad is built for the shape and the row count makes it pay.  A bf16
     input selects the mixed-precision form (bf16 in, bf16 out).  `act` = (seed, salt, p): dropout_p(relu(lin(x))), applied in place on
-    the GEMM's result (csrc/k_train_fused.hip)."""
+    the GEMM's result (csrc/k_train_fused.hip).  `held` = mx8.quantize(x): the backward gets x in this 8-bit form (where
+    da_linear_wgrad_mx8 is built for the shape)."""
     shape = (lin.in_features, lin.out_features)
+    if held is not None and act is None and _mx8_linear(lin):
+        return WideLinearMx8.apply(x, lin.weight, lin.bias, *held)
     if x.dtype == torch.bfloat16:
         if shape in _WGRAD_SHAPES and lin.bias is not None and torch.is_grad_enabled():
             return WideLinearBF16.apply(x, lin.weight, lin.bias, act)

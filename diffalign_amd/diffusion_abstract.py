@@ -46,16 +46,18 @@ class DiscreteDenoisingDiffusion(SamplingMixin, ELBOMixin, TrainingMixin, nn.Mod
                                                          cfg.diffusion.edge_states_to_mask)
         abs_e, abs_x = 0, self.dataset_info.atom_decoder.index('Au')                                   # :67-68
         nn_ = cfg.neuralnet
+        # options of the per-head attention that the reference's configuration does not have
+        head = dict(score_cap=getattr(nn_, 'score_cap', 0.0), attn_scope=getattr(nn_, 'attn_scope', 'all'))
         if nn_.architecture == 'with_y':
             self.model = GraphTransformerWithY(n_layers=nn_.n_layers, input_dims=input_dims, hidden_mlp_dims=nn_.hidden_mlp_dims,
                                                hidden_dims=nn_.hidden_dims, output_dims=output_dims, act_fn_in=nn.ReLU(),
-                                               act_fn_out=nn.ReLU(), improved=nn_.improved, dropout=nn_.dropout)
+                                               act_fn_out=nn.ReLU(), improved=nn_.improved, dropout=nn_.dropout, **head)
         elif nn_.architecture == 'with_y_atommap_number_pos_enc':
             self.model = GraphTransformerWithYAtomMapPosEmb(
                 n_layers=nn_.n_layers, input_dims=input_dims, hidden_mlp_dims=nn_.hidden_mlp_dims, hidden_dims=nn_.hidden_dims,
                 output_dims=output_dims, act_fn_in=nn.ReLU(), act_fn_out=nn.ReLU(), pos_emb_permutations=nn_.pos_emb_permutations,
                 improved=nn_.improved, dropout=nn_.dropout, p_to_r_skip_connection=nn_.p_to_r_skip_connection,
-                p_to_r_init=nn_.p_to_r_init, alignment_type=nn_.alignment_type, input_alignment=nn_.input_alignment)
+                p_to_r_init=nn_.p_to_r_init, alignment_type=nn_.alignment_type, input_alignment=nn_.input_alignment, **head)
         else:
             raise ValueError(f'Unknown architecture: {nn_.architecture}')
         self.ema = None

@@ -24,13 +24,26 @@ class Etoy(nn.Module):
         self.lin = nn.Linear(4 * d, dy)
 
 
+ATTN_SCOPES = ('all', 'nodes', 'side')
+
+
 class NodeEdgeBlock(nn.Module):
     """layers.py:166-202 (parameters); forward is fused into XEyTransformerLayer's HIP path.
     `improved`: the parameters of NodeEdgeBlockImproved (layers.py:49-85) are the same set under the same names (its y_e_mul /
-    y_e_add exist but are unused); only the arithmetic differs (train_forward._node_edge_block_improved)."""
-    def __init__(self, dx, de, dy, n_head, improved=False, **kwargs):
+    y_e_add exist but are unused); only the arithmetic differs (train_forward._node_edge_block_improved).
+    `score_cap`, `scope` (improved only; not in the reference): the head's score s becomes score_cap tanh(s / score_cap) where
+    score_cap > 0; the softmax runs over 'all' keys (the reference: padded ones too), over the 'nodes' that are real, or over the real
+    nodes of the query's own 'side' (product or reactants)."""
+    def __init__(self, dx, de, dy, n_head, improved=False, score_cap=0.0, scope='all', **kwargs):
         super().__init__()
         self.improved = improved
+        if scope not in ATTN_SCOPES:
+            raise ValueError(f'attention scope {scope!r}: one of {ATTN_SCOPES}')
+        if not 0.0 <= float(score_cap) < float('inf'):
+            raise ValueError(f'score_cap = {score_cap}')
+        if not improved and (scope != 'all' or score_cap):
+            raise ValueError('score_cap and scope belong to the per-head attention: improved=True')
+        self.score_cap, self.scope = float(score_cap), scope
         assert dx % n_head == 0, f"dx: {dx} -- nhead: {n_head}"
         self.dx, self.de, self.dy, self.df, self.n_head = dx, de, dy, dx // n_head, n_head
         self.q = Linear(dx, dx); self.k = Linear(dx, dx); self.v = Linear(dx, dx)
@@ -46,11 +59,12 @@ class NodeEdgeBlock(nn.Module):
 class XEyTransformerLayer(nn.Module):
     """layers.py:286-361.  dim_ffy keeps the reference's default 2048 (the model ctor never passes it)."""
     def __init__(self, dx: int, de: int, dy: int, n_head: int, dim_ffX: int = 2048, dim_ffE: int = 128, dim_ffy: int = 2048,
-                 dropout: float = 0.1, layer_norm_eps: float = 1e-5, device=None, dtype=None, improved=False) -> None:
+                 dropout: float = 0.1, layer_norm_eps: float = 1e-5, device=None, dtype=None, improved=False,
+                 score_cap: float = 0.0, scope: str = 'all') -> None:
         super().__init__()
         assert layer_norm_eps == 1e-5
         kw = {'device': device, 'dtype': dtype}
-        self.self_attn = NodeEdgeBlock(dx, de, dy, n_head, improved=improved)                       # layers.py:302
+        self.self_attn = NodeEdgeBlock(dx, de, dy, n_head, improved=improved, score_cap=score_cap, scope=scope)      # layers.py:302
         self.linX1 = Linear(dx, dim_ffX, **kw); self.linX2 = Linear(dim_ffX, dx, **kw)
         self.normX1 = LayerNorm(dx, eps=layer_norm_eps, **kw); self.normX2 = LayerNorm(dx, eps=layer_norm_eps, **kw)
         self.linE1 = Linear(de, dim_ffE, **kw); self.linE2 = Linear(dim_ffE, de, **kw)

@@ -19,8 +19,9 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib as L
+from . import mx8
 from .autograd_ops import (AttnCore, AttnCoreBF16, AddLayerNorm, PoolStats, MaskDense, ResidualLN, ReluDropout, FUSED_WIDTHS, qscale_of,
-                           wide_linear)
+                           wide_linear, feed_forward, head_attention, head_attention_built)
 
 
 # The node (B n rows) and y (B rows) sides of a layer are ~150 launches of a few microseconds each, forward plus backward, beside a
@@ -67,9 +68,15 @@ class _Lanes:
         return ts
 
 
-def _node_edge_block(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False):
+def _hold(x, checkpoint):
+    """x in 8 bits for the backward pass (checkpoint == 'mx8' under autograd), else None."""
+    return mx8.quantize(x) if checkpoint == 'mx8' and torch.is_grad_enabled() else None
+
+
+def _node_edge_block(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False, checkpoint='none'):
     """layers.py:204-284.  `Eb`: E in bf16 (mixed precision): the 256-wide per-pair tensors E1, E2, Z and their gradients are bf16
-    in memory, the three projections bf16 GEMMs with fp32 accumulation; the node and y sides stay fp32."""
+    in memory, the three projections bf16 GEMMs with fp32 accumulation; the node and y sides stay fp32.  checkpoint='mx8': the three
+    projections' inputs are held in 8 bits; E1 and E2 stay, the per-channel softmax is computed again from them."""
     with lanes.on_node():
         Q, K, V = a.q(X) * xm, a.k(X) * xm, a.v(X) * xm
         yea, yem = a.y_e_add(y), a.y_e_mul(y)
@@ -77,11 +84,12 @@ def _node_edge_block(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False
     pE = PoolStats.apply(E)
     bf = Eb is not None and a.dx % 4 == 0 and 256 % (a.dx // 4) == 0
     src = Eb if bf else E
-    E1, E2 = wide_linear(a.e_mul, src), wide_linear(a.e_add, src)
+    held = _hold(src, checkpoint)
+    E1, E2 = wide_linear(a.e_mul, src, held=held), wide_linear(a.e_add, src, held=held)
     lanes.to_pair(Q, K, V, yea, yem)
     Z, wV = (AttnCoreBF16 if bf else AttnCore).apply(Q, K, V, E1, E2, nm_u8, yea, yem, qscale_of(a.dx, a.n_head))
     lanes.to_node(wV, pE)
-    newE = wide_linear(a.e_out, Z)
+    newE = wide_linear(a.e_out, Z, held=_hold(Z, checkpoint))
     if not fused:                     # fused: the mask (and the widening) happen inside the residual block's kernel
         newE = (newE.float() if bf else newE) * em
     with lanes.on_node():
@@ -90,21 +98,62 @@ def _node_edge_block(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False
     return newX, newE, new_y
 
 
-def _node_edge_block_improved(a, X, E, y, nm_u8, xm, em):
+def _node_edge_block_improved(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False, checkpoint='none', groups=None):
     """layers.py:87-164 NodeEdgeBlockImproved: the edge update takes Y without the y FiLM, and attention is ONE softmax per head over the
-    head's summed scores (the plain block has one per channel).  Off in both align_* experiments (configs/neuralnet/transformer.yaml:15);
-    written in torch ops over the library GEMMs -- it has no fused HIP form, inference runs this same code without a graph."""
-    B, n, dx = X.shape
-    H, df = a.n_head, a.df
-    Q, K, V = a.q(X) * xm, a.k(X) * xm, a.v(X) * xm
-    Y = Q[:, :, None, :] * K[:, None, :, :] * qscale_of(a.dx, a.n_head)                        # (B,i,j,dx)
-    Y = Y * (wide_linear(a.e_mul, E) * em + 1) + wide_linear(a.e_add, E) * em                 # :115-122
-    newE = wide_linear(a.e_out, Y) * em                                                       # :123-125
-    attn = torch.softmax(Y.reshape(B, n, n, H, df).sum(-1), dim=2)                            # :128-130 (over keys, no mask)
-    wV = torch.einsum('bijh,bjhf->bihf', attn, V.reshape(B, n, H, df)).reshape(B, n, dx)      # :132-141
-    newX = a.x_out(a.y_x_add(y)[:, None, :] + (a.y_x_mul(y)[:, None, :] + 1) * wV) * xm       # :148-153
-    new_y = a.y_out(y + a.x_y.lin(PoolStats.apply(X)) + a.e_y.lin(PoolStats.apply(E)))       # :157-161
+    head's summed scores (the plain block has one per channel); head_attention is its core.  Off in both align_* experiments
+    (configs/neuralnet/transformer.yaml:15); inference runs this same code without a graph.  Arguments as _node_edge_block's; `groups`: the
+    softmax's groups of keys (NodeEdgeBlock.scope), None = all keys."""
+    with lanes.on_node():
+        Q, K, V = a.q(X) * xm, a.k(X) * xm, a.v(X) * xm
+        pX = PoolStats.apply(X)
+    pE = PoolStats.apply(E)
+    src = E if Eb is None else Eb
+    held = _hold(src, checkpoint)
+    E1, E2 = wide_linear(a.e_mul, src, held=held), wide_linear(a.e_add, src, held=held)       # :115-122
+    lanes.to_pair(Q, K, V)
+    if head_attention_built(a.dx, a.n_head):
+        Y, wV = head_attention(Q, K, V, E1, E2, nm_u8, a.n_head, cap=a.score_cap, groups=groups,
+                               checkpoint=checkpoint if a.dx % mx8.GROUP == 0 else 'none')
+    else:
+        Y, wV = _head_attention_torch(a, Q, K, V, E1, E2, em, groups)
+    lanes.to_node(wV, pE)
+    newE = wide_linear(a.e_out, Y, held=_hold(Y, checkpoint))                                 # :123-125
+    if not fused:
+        newE = newE.float() * em
+    with lanes.on_node():
+        newX = a.x_out(a.y_x_add(y)[:, None, :] + (a.y_x_mul(y)[:, None, :] + 1) * wV) * xm   # :148-153
+        new_y = a.y_out(y + a.x_y.lin(pX) + a.e_y.lin(pE))                                    # :157-161
     return newX, newE, new_y
+
+
+def _head_attention_torch(a, Q, K, V, E1, E2, em, groups):
+    """head_attention for head widths it is not built for, in torch operations."""
+    B, n, dx = Q.shape
+    H, df = a.n_head, a.df
+    Y = Q[:, :, None, :] * K[:, None, :, :] * qscale_of(dx, H)                                 # (B,i,j,dx)
+    Y = Y * (E1.float() * em + 1) + E2.float() * em                                           # :115-122
+    S = Y.reshape(B, n, n, H, df).sum(-1)
+    if a.score_cap > 0:
+        S = a.score_cap * torch.tanh(S / a.score_cap)
+    if groups is not None:
+        on = ((groups[:, :, None] == groups[:, None, :]) & (groups >= 0)[:, :, None])[..., None]
+        some = on.any(2, keepdim=True)                                                        # a row without a key: 0
+        attn = torch.softmax(torch.where(on | ~some, S, float('-inf')), dim=2) * some
+    else:
+        attn = torch.softmax(S, dim=2)                                                        # :128-130 (over keys, no mask)
+    wV = torch.einsum('bijh,bjhf->bihf', attn, V.reshape(B, n, H, df)).reshape(B, n, dx)      # :132-141
+    return Y.to(E1.dtype), wV
+
+
+def _attn_groups(m, node_mask, mol_assignments):
+    """(B,n) int32 groups of keys for the module's attention scope (NodeEdgeBlock.scope), None: all keys."""
+    scope = m.tf_layers[0].self_attn.scope if len(m.tf_layers) else 'all'
+    if scope == 'all':
+        return None
+    side = torch.zeros_like(node_mask, dtype=torch.int32)
+    if scope == 'side':       # 1 = product (the molecule with the largest number, as in align_index), 0 = reactants
+        side = (mol_assignments == mol_assignments.max(-1, keepdim=True).values).int()
+    return torch.where(node_mask.bool(), side, -1).int()
 
 
 # Fused residual blocks (csrc/k_train_fused.hip: mask + dropout + add + LayerNorm (+ bf16 copy for the next GEMM) in one kernel each
@@ -123,7 +172,7 @@ def _dropout_seed(dev):
     return st.clone()
 
 
-def _layer(layer, X, E, y, nm_u8, xm, em, training, bf16=False, lanes=None, Eb=None, fuse=None):
+def _layer(layer, X, E, y, nm_u8, xm, em, training, bf16=False, lanes=None, Eb=None, fuse=None, checkpoint='none', groups=None):
     """layers.py:330-361 (post-LN residual blocks; dropout only in train mode).  X and y live on lanes.node, E on lanes.pair.
     `fuse` = (seed tensor, salt base) selects the fused residual blocks; then `Eb` carries E in bf16 between layers (mixed precision)
     and the layer returns (X, E, y, Eb)."""
@@ -134,7 +183,10 @@ def _layer(layer, X, E, y, nm_u8, xm, em, training, bf16=False, lanes=None, Eb=N
         seed, salt = fuse
         if bf16 and Eb is None:
             Eb = E.to(torch.bfloat16)
-        nX, nE, ny = _node_edge_block(layer.self_attn, X, E, y, nm_u8, xm, em, Eb if bf16 else None, lanes, fused=True)
+        if layer.self_attn.improved:
+            nX, nE, ny = _node_edge_block_improved(layer.self_attn, X, E, y, nm_u8, xm, em, Eb if bf16 else None, lanes, True, checkpoint, groups)
+        else:
+            nX, nE, ny = _node_edge_block(layer.self_attn, X, E, y, nm_u8, xm, em, Eb if bf16 else None, lanes, True, checkpoint)
         with lanes.on_node():
             X, _ = ResidualLN.apply(X, nX, nm_u8, 0, n, layer.normX1.weight, layer.normX1.bias, seed, salt + 0, p, False)   # nX is masked already
             y, _ = ResidualLN.apply(y, ny, nm_u8, 0, n, layer.norm_y1.weight, layer.norm_y1.bias, seed, salt + 1, p, False)
@@ -143,13 +195,11 @@ def _layer(layer, X, E, y, nm_u8, xm, em, training, bf16=False, lanes=None, Eb=N
             h = ReluDropout.apply(layer.lin_y1(y), seed, salt + 4, p)
             y, _ = ResidualLN.apply(y, layer.lin_y2(h), nm_u8, 0, n, layer.norm_y2.weight, layer.norm_y2.bias, seed, salt + 5, p, False)
         E, Eb = ResidualLN.apply(E, nE, nm_u8, 2, n, layer.normE1.weight, layer.normE1.bias, seed, salt + 6, p, bf16)
-        h = wide_linear(layer.linE1, Eb if bf16 else E, act=(seed, salt + 7, p))
-        E, Eb = ResidualLN.apply(E, wide_linear(layer.linE2, h), nm_u8, 0, n, layer.normE2.weight, layer.normE2.bias, seed, salt + 8, p, bf16)
+        h = feed_forward(layer.linE1, layer.linE2, Eb if bf16 else E, (seed, salt + 7, p), checkpoint)
+        E, Eb = ResidualLN.apply(E, h, nm_u8, 0, n, layer.normE2.weight, layer.normE2.bias, seed, salt + 8, p, bf16)
         return X, E, y, Eb
     if layer.self_attn.improved:
-        lanes.to_pair(X, y)
-        nX, nE, ny = _node_edge_block_improved(layer.self_attn, X, E, y, nm_u8, xm, em)
-        lanes.to_node(nX, ny)
+        nX, nE, ny = _node_edge_block_improved(layer.self_attn, X, E, y, nm_u8, xm, em, None, lanes, groups=groups)
     else:
         nX, nE, ny = _node_edge_block(layer.self_attn, X, E, y, nm_u8, xm, em, E.to(torch.bfloat16) if bf16 else None, lanes)
     with lanes.on_node():
@@ -166,11 +216,12 @@ def _layer(layer, X, E, y, nm_u8, xm, em, training, bf16=False, lanes=None, Eb=N
     return X, E, y, None
 
 
-def _fusable(layer, X, E, y):
-    """the fused blocks are built for row widths 16..256 (powers of two) and hidden sizes that are multiples of 4"""
+def _fusable(layer, X, E, y, checkpoint='none'):
+    """the fused blocks are built for row widths 16..256 (powers of two) and hidden sizes that are multiples of 4; the improved block takes
+    them together with the 8-bit activations"""
     ok = X.shape[-1] in FUSED_WIDTHS and E.shape[-1] in FUSED_WIDTHS and y.shape[-1] in FUSED_WIDTHS
     hid = (layer.linX1.out_features, layer.linE1.out_features, layer.lin_y1.out_features)
-    return ok and not layer.self_attn.improved and all(h % 4 == 0 for h in hid)
+    return ok and (checkpoint == 'mx8' or not layer.self_attn.improved) and all(h % 4 == 0 for h in hid)
 
 
 def align_index(atom_map_numbers, mol_assignments, alignment_type='correct'):
@@ -221,6 +272,13 @@ def aligned_product_features(X, E, atom_map_numbers, mol_assignments, kx, ke, al
 PRECISION = _os.environ.get('DA_TRAIN_PRECISION', 'fp32')
 
 
+# 'none' (default: the backward gets every activation as the forward had it) or 'mx8': the inputs of the per-pair Linears of the layers, and in the
+# improved block the attention's E1, are held in 8 bits between the two passes (mx8.py).  The forward's values do not change; the gradients of
+# those weights, and dQ and dK of the per-head attention, see the rounded values.  Goes with the fused residual blocks.  Set per module
+# (`module.train_checkpoint = 'mx8'`) or process-wide here / by DA_TRAIN_CHECKPOINT.
+CHECKPOINT = _os.environ.get('DA_TRAIN_CHECKPOINT', 'none')
+
+
 def forward_train(m, X, E, y, node_mask, atom_map_numbers=None, pos_encodings=None, mol_assignments=None, precision=None):
     """Differentiable forward of the denoiser module `m`; returns (X logits, E logits, y) like the module's forward.
     `precision` overrides the module's / the process's training precision (the fp32 inference mode passes 'fp32')."""
@@ -228,6 +286,11 @@ def forward_train(m, X, E, y, node_mask, atom_map_numbers=None, pos_encodings=No
     if bf16 not in ('fp32', 'bf16'):
         raise ValueError(f"train precision {bf16!r}: 'fp32' or 'bf16'")
     bf16 = bf16 == 'bf16'
+    checkpoint = getattr(m, 'train_checkpoint', None) or CHECKPOINT
+    if checkpoint not in ('none', 'mx8'):
+        raise ValueError(f"train checkpoint {checkpoint!r}: 'none' or 'mx8'")
+    if not (m.training and torch.is_grad_enabled()):
+        checkpoint = 'none'
     if not X.is_cuda:
         raise L.DiffAlignHipError('denoiser inputs must be on a HIP device (no CPU fallback)')
     X, E, y = X.float(), E.float(), y.float()
@@ -247,12 +310,15 @@ def forward_train(m, X, E, y, node_mask, atom_map_numbers=None, pos_encodings=No
         Xh = Xh + pos_encodings.float()
     lanes = _Lanes(X.device, SIDE_STREAM and getattr(m, 'train_side_stream', True))
     fused = FUSED and getattr(m, 'train_fused', True)
+    if checkpoint == 'mx8' and not fused:
+        raise ValueError("train checkpoint 'mx8' goes with the fused residual blocks (train_fused)")
+    groups = _attn_groups(m, node_mask, mol_assignments)
     seed = _dropout_seed(X.device) if fused and m.training else None
     lanes.to_node(Xh, yh, xm, seed)
     Eb = None
     for k, layer in enumerate(m.tf_layers):
-        fuse = (seed, 16 * k) if fused and _fusable(layer, Xh, Eh, yh) else None
-        Xh, Eh, yh, Eb = _layer(layer, Xh, Eh, yh, nm_u8, xm, em, m.training, bf16, lanes, Eb, fuse)
+        fuse = (seed, 16 * k) if fused and _fusable(layer, Xh, Eh, yh, checkpoint) else None
+        Xh, Eh, yh, Eb = _layer(layer, Xh, Eh, yh, nm_u8, xm, em, m.training, bf16, lanes, Eb, fuse, checkpoint, groups)
     lanes.to_pair(Xh, yh)
     kx, ke, ky = m.out_dim_X, m.out_dim_E, m.out_dim_y
     Xo = m.mlp_out_X(Xh) + X[..., :kx]

@@ -15,9 +15,9 @@ from .layers import XEyTransformerLayer
 
 class _DenoiserBase(nn.Module):
     def _build(self, n_layers, input_dims, hidden_mlp_dims, hidden_dims, output_dims, act_fn_in, act_fn_out, improved,
-               dropout):
+               dropout, score_cap=0.0, attn_scope='all'):
         self.n_layers = n_layers
-        self.improved = bool(improved)       # NodeEdgeBlockImproved has no fused inference kernels: forward() always takes train_forward's path
+        self.improved = bool(improved)       # NodeEdgeBlockImproved has no fused layer kernel: forward() always takes train_forward's path
         self.n_head = hidden_dims['n_head']
         self.out_dim_X, self.out_dim_E, self.out_dim_y = output_dims['X'], output_dims['E'], output_dims['y']
         if not isinstance(act_fn_in, nn.ReLU) or not isinstance(act_fn_out, nn.ReLU):
@@ -28,7 +28,8 @@ class _DenoiserBase(nn.Module):
         self.mlp_in_y = mk(input_dims['y'], hidden_mlp_dims['y'], hidden_dims['dy'], True)
         self.tf_layers = nn.ModuleList([XEyTransformerLayer(dx=hidden_dims['dx'], de=hidden_dims['de'], dy=hidden_dims['dy'],
                                                             n_head=hidden_dims['n_head'], dim_ffX=hidden_dims['dim_ffX'],
-                                                            dim_ffE=hidden_dims['dim_ffE'], improved=improved, dropout=dropout)
+                                                            dim_ffE=hidden_dims['dim_ffE'], improved=improved, dropout=dropout,
+                                                            score_cap=score_cap, scope=attn_scope)
                                         for _ in range(n_layers)])
         self.mlp_out_X = mk(hidden_dims['dx'], hidden_mlp_dims['X'], output_dims['X'], False)
         self.mlp_out_E = mk(hidden_dims['de'], hidden_mlp_dims['E'], output_dims['E'], False)
@@ -83,9 +84,11 @@ class _DenoiserBase(nn.Module):
 
 class GraphTransformerWithY(_DenoiserBase):
     def __init__(self, n_layers: int, input_dims: dict, hidden_mlp_dims: dict, hidden_dims: dict, output_dims: dict,
-                 act_fn_in=nn.ReLU(), act_fn_out=nn.ReLU(), improved=False, dropout=0.1):
+                 act_fn_in=nn.ReLU(), act_fn_out=nn.ReLU(), improved=False, dropout=0.1, score_cap=0.0, attn_scope='all'):
         super().__init__()
-        self._build(n_layers, input_dims, hidden_mlp_dims, hidden_dims, output_dims, act_fn_in, act_fn_out, improved, dropout)
+        if attn_scope == 'side':
+            raise ValueError("attn_scope='side' needs the molecule assignments of GraphTransformerWithYAtomMapPosEmb")
+        self._build(n_layers, input_dims, hidden_mlp_dims, hidden_dims, output_dims, act_fn_in, act_fn_out, improved, dropout, score_cap, attn_scope)
 
     def forward(self, X, E, y, node_mask, step=None):
         self._check(X)
@@ -110,7 +113,8 @@ def _join_inputs(step):
 class GraphTransformerWithYAtomMapPosEmb(_DenoiserBase):
     def __init__(self, n_layers: int, input_dims: dict, hidden_mlp_dims: dict, hidden_dims: dict, output_dims: dict,
                  act_fn_in=nn.ReLU(), act_fn_out=nn.ReLU(), pos_emb_permutations: int = 0, improved=False, dropout=0.1,
-                 p_to_r_skip_connection=False, p_to_r_init=10., alignment_type='old', input_alignment=False):
+                 p_to_r_skip_connection=False, p_to_r_init=10., alignment_type='old', input_alignment=False, score_cap=0.0,
+                 attn_scope='all'):
         super().__init__()
         if input_alignment:                                              # :575-580: the aligned product features widen both inputs
             input_dims = dict(input_dims)
@@ -122,7 +126,7 @@ class GraphTransformerWithYAtomMapPosEmb(_DenoiserBase):
         self.p_to_r_skip_connection = p_to_r_skip_connection
         self.alignment_type = alignment_type
         self.input_alignment = input_alignment
-        self._build(n_layers, input_dims, hidden_mlp_dims, hidden_dims, output_dims, act_fn_in, act_fn_out, improved, dropout)
+        self._build(n_layers, input_dims, hidden_mlp_dims, hidden_dims, output_dims, act_fn_in, act_fn_out, improved, dropout, score_cap, attn_scope)
         if p_to_r_skip_connection:
             self.skip_scaling = nn.Parameter(torch.tensor([p_to_r_init], dtype=torch.float))
             self.skip_scaling_2 = nn.Parameter(torch.tensor([p_to_r_init], dtype=torch.float))

@@ -71,3 +71,19 @@ def test_c_entries_refuse_before_any_launch():
     assert bwd() == -1 and b'workspace' in lib.da_last_error()
     assert bwd(E1=0) == -1 and bwd(c=p, sc=p) == -1 and bwd(E1=0, c=p) == -1 and bwd(dY=0) == -1 and bwd(H=5) == -3 and bwd(B=0) == 0
     assert bwd(dQ=8) == -1 and b'unaligned' in lib.da_last_error()
+
+
+def test_model_options_are_checked():
+    import torch.nn as nn
+    from diffalign_amd.layers import NodeEdgeBlock
+    from diffalign_amd.transformer_model_with_y import GraphTransformerWithY
+    for kw in (dict(score_cap=3.0), dict(scope='nodes'), dict(improved=True, scope='molecule'), dict(improved=True, score_cap=-1.0),
+               dict(improved=True, score_cap=float('inf')), dict(improved=True, score_cap=float('nan'))):
+        with pytest.raises(ValueError):
+            NodeEdgeBlock(64, 32, 32, 4, **kw)
+    blk = NodeEdgeBlock(64, 32, 32, 4, improved=True, score_cap=3.0, scope='side')
+    assert blk.score_cap == 3.0 and blk.scope == 'side' and set(blk.state_dict()) == set(NodeEdgeBlock(64, 32, 32, 4).state_dict())
+    dims = dict(X=16, E=16, y=16)
+    with pytest.raises(ValueError):
+        GraphTransformerWithY(1, dims, dims, dict(dx=16, de=16, dy=16, n_head=2, dim_ffX=16, dim_ffE=16), dims, nn.ReLU(), nn.ReLU(), improved=True,
+                              attn_scope='side')
