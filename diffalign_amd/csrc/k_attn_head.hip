@@ -47,10 +47,10 @@ struct HeadArgs {
 };
 
 #define OOB 0x80000000u                 // past every descriptor's range, also with a row's offset added (the host keeps both below 2^31)
-// cache policy of the streams that pass once (E1, E2, Y, dY, dE1, dE2): non-temporal for bf16, so that K and V keep the L2 (forward B = 16,
-// n = 140 96 -> 88 us, backward n = 300 565 -> 532 us); fp32 takes two instructions for a lane's 8 channels, each touching half of
-// every 64 bytes, and wants the line kept for the second (forward / backward n = 93 49 / 49 us, non-temporal 52 / 55)
-template <class TE> constexpr int nt() { return sizeof(TE) == 2 ? 2 : 0; }
+// cache policy of the streams that pass once (E1, E2, Y, dY, dE1, dE2): non-temporal where a lane's channels are one 16-byte access, so that K
+// and V keep the L2 (bf16: forward B = 16, n = 140 96 -> 88 us, backward n = 300 565 -> 532 us; fp32: 169 -> 158 and 518 -> 498 us).  Eight
+// fp32 channels take two accesses that share every 64 bytes, and want the line kept for the second (n = 93: 49 / 49 us, non-temporal 52 / 55)
+template <class TE, int C> constexpr int nt() { return sizeof(TE) * C == 16 ? 2 : 0; }
 template <class TE, int C> struct Raw { unsigned w[sizeof(TE) * C / 4]; };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, unsigned bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
@@ -84,16 +84,16 @@ template <class TE, int C>
 __device__ __forceinline__ void bst(__amdgpu_buffer_rsrc_t r, unsigned off, const float (&v)[C]) {
   if constexpr (sizeof(TE) == 2 && C == 8) {
     const u32x4 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
-    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, nt<TE>());
+    __builtin_amdgcn_raw_buffer_store_b128(o, r, off, 0, nt<TE, C>());
   } else if constexpr (sizeof(TE) == 2) {
     const u32x2 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-    __builtin_amdgcn_raw_buffer_store_b64(o, r, off, 0, nt<TE>());
+    __builtin_amdgcn_raw_buffer_store_b64(o, r, off, 0, nt<TE, C>());
   } else {
 #pragma unroll
     for (int k = 0; k < C; k += 4) {
       const u32x4 o = {__builtin_bit_cast(unsigned, v[k]), __builtin_bit_cast(unsigned, v[k + 1]), __builtin_bit_cast(unsigned, v[k + 2]),
                        __builtin_bit_cast(unsigned, v[k + 3])};
-      __builtin_amdgcn_raw_buffer_store_b128(o, r, off + 4 * k, 0, nt<TE>());
+      __builtin_amdgcn_raw_buffer_store_b128(o, r, off + 4 * k, 0, nt<TE, C>());
     }
   }
 }
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
   const unsigned row_c = (unsigned)(n * dx), row_e = row_c * es;
   auto fetch = [&](int t, unsigned eo) {
     const unsigned o = mi[t] ? eo : OOB, so = mi[t] ? t * row_e : 0;
-    bld<nt<TE>()>(r1, o, e1n[t].w, so); bld<nt<TE>()>(r2, o, e2n[t].w, so);
+    bld<nt<TE, C>()>(r1, o, e1n[t].w, so); bld<nt<TE, C>()>(r2, o, e2n[t].w, so);
   };
   auto key_off = [&](int j, uint8_t mj) { return act & (j < n) & (mj != 0) ? (unsigned)(j * dx + c) * es : OOB; };
   const int jf = w * NS + slot;
@@ -209,8 +209,8 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
         const unsigned sb = mx8_scale(C == 8 ? quad_max(mb) : oct_max(mb));
         const float inv = mx8_inv(sb);
         const unsigned w0 = mx8_pack4<false>(e1[0], e1[1], e1[2], e1[3], inv), co = oC + t * row_c;
-        if constexpr (C == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)}, rc, co, 0, nt<TE>());
-        else __builtin_amdgcn_raw_buffer_store_b32(w0, rc, co, 0, nt<TE>());
+        if constexpr (C == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2{w0, mx8_pack4<false>(e1[4], e1[5], e1[6], e1[7], inv)}, rc, co, 0, nt<TE, C>());
+        else __builtin_amdgcn_raw_buffer_store_b32(w0, rc, co, 0, nt<TE, C>());
         __builtin_amdgcn_raw_buffer_store_b8((uint8_t)sb, rcs, oCs + t * (row_c / MX8_GROUP), 0, 0);
       }
       s = head_sum<HLOG>(s);
@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
 // stays in registers over the chunk.  k_attn_head_fold adds the partial results in order (no atomics: the sums do not depend on timing).
 #define HEAD_NW 8
 // rows a wave: what its registers hold without spilling (two waves a SIMD)
-template <class TY> __host__ __device__ constexpr int head_rw() { return sizeof(TY) == 2 ? 4 : 2; }
+__host__ __device__ constexpr int head_rw(bool bf16, int C) { return bf16 || C == 4 ? 4 : 2; }
 template <class TY, int C, int HLOG, bool MX8>
 __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
-  constexpr int RW = head_rw<TY>(), NW = HEAD_NW;
+  constexpr int RW = head_rw(sizeof(TY) == 2, C), NW = HEAD_NW;
   extern __shared__ float s_kv[];                                       // [2][NW][NS][2][dx]
   const int n = a.n, dx = a.dx, H = a.H;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, slot = lane >> a.lp_log, li = lane & ((1 << a.lp_log) - 1);
@@ -332,9 +332,9 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
   const unsigned row_c = (unsigned)(n * dx), row_e = row_c * es;
   auto fetch = [&](int t, const Off& o) {
     const bool in = t < rows;
-    bld<nt<TY>()>(r1, mi[t] ? o.e1 : OOB, op[t].e1, mi[t] ? t * (MX8 ? row_c : row_e) : 0);
+    bld<nt<TY, C>()>(r1, mi[t] ? o.e1 : OOB, op[t].e1, mi[t] ? t * (MX8 ? row_c : row_e) : 0);
     if constexpr (MX8) op[t].sc = __builtin_amdgcn_raw_buffer_load_b8(rsc, mi[t] ? o.sc : OOB, mi[t] ? t * (row_c / MX8_GROUP) : 0, 0);
-    bld<nt<TY>()>(ry, in ? o.y : OOB, op[t].dy.w, in ? t * row_e : 0);
+    bld<nt<TY, C>()>(ry, in ? o.y : OOB, op[t].dy.w, in ? t * row_e : 0);
     op[t].s = __builtin_amdgcn_raw_buffer_load_b32(rS, in ? o.s : OOB, in ? (unsigned)(t * n * H) * 4 : 0, 0);
   };
   uint8_t m0 = meta(j_lo + slot), m1 = meta(j_lo + slot + NS);
@@ -455,11 +455,12 @@ __global__ void __launch_bounds__(256) k_attn_head_fold(const float4* __restrict
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// channels per lane and lanes per head; false: not built
-static bool head_shape(int dx, int H, int* C, int* hlog, int* lp_log) {
+// channels per lane and lanes per head; false: not built.  16 bytes of the pair tensors per lane (8 bf16, 4 fp32 channels) where a pair then fits
+// 64 lanes and a head 16: fp32 B = 16, n = 140 backward + fold 263 us, with 8 channels 309 us
+static bool head_shape(int dx, int H, bool bf16, int* C, int* hlog, int* lp_log) {
   if (dx < 4 || H < 1 || dx % H) return false;
   const int df = dx / H;
-  *C = df == 4 ? 4 : 8;
+  *C = df == 4 || (!bf16 && dx <= 256 && df <= 64) ? 4 : 8;
   int l = 0;
   while ((*C << l) < df) ++l;
   if ((*C << l) != df || l > 4 || dx / *C > 64) return false;
@@ -472,8 +473,8 @@ static bool head_shape(int dx, int H, int* C, int* hlog, int* lp_log) {
 // backward: row blocks, and the keys cut into chunks so that the workgroups fill the 256 CUs in whole rounds.  One workgroup runs on a CU at a
 // time (its registers); it takes its chunk's steps and HEAD_FIXED more for its beginning and end.
 #define HEAD_FIXED 6
-static void head_chunks(int B, int n, int lp_log, bool bf16, int* nib, int* njc, int* jchunk) {
-  const int NS = 64 >> lp_log, rows = HEAD_NW * (bf16 ? head_rw<bf16_t>() : head_rw<float>());
+static void head_chunks(int B, int n, int C, int lp_log, bool bf16, int* nib, int* njc, int* jchunk) {
+  const int NS = 64 >> lp_log, rows = HEAD_NW * head_rw(bf16, C);
   *nib = (n + rows - 1) / rows;
   long long best = -1;
   for (int want = 1; want <= 64 && (want == 1 || (want - 1) * 4 * NS < n); ++want) {
@@ -504,16 +505,16 @@ static void bwd_launch(const HeadArgs& a, bool mx8, hipStream_t s) {
   if (mx8) k_attn_head_bwd<TY, C, HLOG, true><<<grid, 64 * HEAD_NW, lds, s>>>(a);
   else k_attn_head_bwd<TY, C, HLOG, false><<<grid, 64 * HEAD_NW, lds, s>>>(a);
 }
-template <class T, class F>
-static void by_shape(int C, int hlog, F f) {
-  if (C == 4) f(std::integral_constant<int, 4>{}, std::integral_constant<int, 0>{});
-  else switch (hlog) {
-    case 0: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 0>{}); break;
-    case 1: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{}); break;
-    case 2: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{}); break;
-    case 3: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 3>{}); break;
-    default: f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}); break;
-  }
+// f(type, channels per lane, log2 of the lanes per head)
+template <int C, int L> struct Shape { static constexpr int c = C, hlog = L; };
+template <class F>
+static void by_shape(bool bf16, int C, int hlog, F f) {
+#define S(T, C, L) f((T*)nullptr, Shape<C, L>{})
+  if (C == 4 && bf16) S(bf16_t, 4, 0);                                  // (4 channels per head)
+  else if (C == 4) switch (hlog) { case 0: S(float, 4, 0); break; case 1: S(float, 4, 1); break; case 2: S(float, 4, 2); break; case 3: S(float, 4, 3); break; default: S(float, 4, 4); }
+  else if (bf16) switch (hlog) { case 0: S(bf16_t, 8, 0); break; case 1: S(bf16_t, 8, 1); break; case 2: S(bf16_t, 8, 2); break; case 3: S(bf16_t, 8, 3); break; default: S(bf16_t, 8, 4); }
+  else switch (hlog) { case 0: S(float, 8, 0); break; case 1: S(float, 8, 1); break; case 2: S(float, 8, 2); break; case 3: S(float, 8, 3); break; default: S(float, 8, 4); }
+#undef S
 }
 static bool al16(std::initializer_list<const void*> ps) {
   uintptr_t v = 0;
@@ -521,9 +522,9 @@ static bool al16(std::initializer_list<const void*> ps) {
   return (v & 15) == 0;
 }
 // sizes both passes take: the descriptors' ranges and offsets are 32-bit (4 rows of a graph's pairs), the grid one-dimensional
-static int head_sizes(const char* who, int B, int n, int dx, int H, int* C, int* hlog, int* lp_log) {
+static int head_sizes(const char* who, int B, int n, int dx, int H, bool bf16, int* C, int* hlog, int* lp_log) {
   DA_CHECK_ARG(B >= 0 && n >= 0 && dx >= 1 && H >= 1, "%s: B = %d, n = %d, dx = %d, n_head = %d", who, B, n, dx, H);
-  if (!head_shape(dx, H, C, hlog, lp_log)) {
+  if (!head_shape(dx, H, bf16, C, hlog, lp_log)) {
     da_set_error("%s: dx = %d with %d heads not built (channels per head 4, 8, 16, .. 128; dx <= 512, 256 with 4 channels per head)", who, dx, H);
     return DA_ERR_UNSUPPORTED;
   }
@@ -538,7 +539,7 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
                      int n, int dx, int n_head, void* stream) {
   HeadArgs a = {};
   int C, hlog;
-  if (int rc = head_sizes("da_attn_head_fwd", B, n, dx, n_head, &C, &hlog, &a.lp_log)) return rc;
+  if (int rc = head_sizes("da_attn_head_fwd", B, n, dx, n_head, e_bf16 != 0, &C, &hlog, &a.lp_log)) return rc;
   if (B == 0 || n == 0) return DA_OK;
   DA_CHECK_ARG(Q && K && V && E1 && E2 && node_mask && Y && wV, "da_attn_head_fwd: null pointer");
   DA_CHECK_ARG((S == nullptr) == (stat == nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr) && (!E1_codes || S),
@@ -548,9 +549,8 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
   DA_CHECK_ARG(al16({Q, K, V, E1, E2, Y, wV, E1_codes}) && ((uintptr_t)stat & 7) == 0 && ((uintptr_t)S & 3) == 0, "da_attn_head_fwd: unaligned tensor (16 bytes)");
   a.Q = Q; a.K = K; a.V = V; a.E1 = E1; a.E2 = E2; a.nm = node_mask; a.grp = groups; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx; a.H = n_head;
   a.Y = Y; a.wV = wV; a.S = S; a.stat = stat; a.q1 = (uint8_t*)E1_codes; a.q1s = E1_scales; a.B = B;
-  by_shape<void>(C, hlog, [&](auto c, auto h) {
-    if (e_bf16) fwd_launch<bf16_t, decltype(c)::value, decltype(h)::value>(a, S != nullptr, E1_codes != nullptr, (hipStream_t)stream);
-    else fwd_launch<float, decltype(c)::value, decltype(h)::value>(a, S != nullptr, E1_codes != nullptr, (hipStream_t)stream);
+  by_shape(e_bf16 != 0, C, hlog, [&](auto* t, auto sh) {
+    fwd_launch<std::remove_pointer_t<decltype(t)>, sh.c, sh.hlog>(a, S != nullptr, E1_codes != nullptr, (hipStream_t)stream);
   });
   DA_CHECK_LAUNCH("da_attn_head_fwd");
   return DA_OK;
@@ -558,9 +558,9 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
 
 long long da_attn_head_bwd_workspace(int B, int n, int dx, int n_head, int dy_bf16) {
   int C, hlog, lp, nib, njc, jchunk;
-  if (B < 0 || n < 0 || !head_shape(dx, n_head, &C, &hlog, &lp)) return -1;
+  if (B < 0 || n < 0 || !head_shape(dx, n_head, dy_bf16 != 0, &C, &hlog, &lp)) return -1;
   if (B == 0 || n == 0) return 0;
-  head_chunks(B, n, lp, dy_bf16 != 0, &nib, &njc, &jchunk);
+  head_chunks(B, n, C, lp, dy_bf16 != 0, &nib, &njc, &jchunk);
   return (long long)sizeof(float) * ((nib > 1 ? 2LL * nib : 0) + (njc > 1 ? njc : 0)) * B * n * dx;
 }
 
@@ -570,7 +570,7 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
                      long long workspace_bytes, int B, int n, int dx, int n_head, void* stream) {
   HeadArgs a = {};
   int C, hlog;
-  if (int rc = head_sizes("da_attn_head_bwd", B, n, dx, n_head, &C, &hlog, &a.lp_log)) return rc;
+  if (int rc = head_sizes("da_attn_head_bwd", B, n, dx, n_head, dy_bf16 != 0, &C, &hlog, &a.lp_log)) return rc;
   if (B == 0 || n == 0) return DA_OK;
   DA_CHECK_ARG(Q && K && V && node_mask && wV && S && stat && dY && dwV && dQ && dK && dV && dE1 && dE2, "da_attn_head_bwd: null pointer");
   DA_CHECK_ARG((E1 != nullptr) != (E1_codes != nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr),
@@ -583,17 +583,14 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
   DA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "da_attn_head_bwd: workspace too small");
   a.Q = Q; a.K = K; a.V = V; a.E1 = E1_codes ? E1_codes : E1; a.E1s = E1_scales; a.nm = node_mask; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx;
   a.H = n_head; a.wV = (float*)wV; a.S = (float*)S; a.stat = (float*)stat; a.dY = dY; a.dwV = dwV; a.dE1 = dE1; a.dE2 = dE2; a.B = B;
-  head_chunks(B, n, a.lp_log, dy_bf16 != 0, &a.nib, &a.njc, &a.jchunk);
+  head_chunks(B, n, C, a.lp_log, dy_bf16 != 0, &a.nib, &a.njc, &a.jchunk);
   const size_t one = (size_t)B * n * dx;
   float* ws = (float*)workspace;
   a.dKp = dK; a.dVp = dV; a.dQp = dQ;
   if (a.nib > 1) { a.dKp = ws; a.dVp = ws + a.nib * one; ws += 2 * a.nib * one; }
   if (a.njc > 1) a.dQp = ws;
   hipStream_t s = (hipStream_t)stream;
-  by_shape<void>(C, hlog, [&](auto c, auto h) {
-    if (dy_bf16) bwd_launch<bf16_t, decltype(c)::value, decltype(h)::value>(a, E1_codes != nullptr, s);
-    else bwd_launch<float, decltype(c)::value, decltype(h)::value>(a, E1_codes != nullptr, s);
-  });
+  by_shape(dy_bf16 != 0, C, hlog, [&](auto* t, auto sh) { bwd_launch<std::remove_pointer_t<decltype(t)>, sh.c, sh.hlog>(a, E1_codes != nullptr, s); });
   if (a.nib > 1 || a.njc > 1) {
     const long long quads = (long long)one / 4;
     const unsigned gx = (unsigned)((quads + 255) / 256);
