@@ -140,6 +140,11 @@ _held = []
 
 def check(rc: int, what: str) -> None:
     _held.clear()
+    raise_on(rc, what)
+
+
+def raise_on(rc: int, what: str) -> None:
+    """check() for callers that hold their tensors themselves: leaves what other threads hold alone."""
     if rc != 0:
         raise DiffAlignHipError(f'{what} failed (rc={rc}): {lib().da_last_error().decode()}')
 

@@ -128,7 +128,7 @@ class WideLinearMx8(Function):
     def backward(ctx, dy):
         codes, scales, w = ctx.saved_tensors
         dy = dy.contiguous()
-        dW, db = mx8.linear_wgrad(mx8.Mx8(codes, scales), dy)
+        dW, db = mx8.linear_wgrad(mx8.Mx8(codes, scales), dy) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
         return (dy @ w if ctx.needs_input_grad[0] else None), dW, db, None, None
 
 
@@ -158,14 +158,15 @@ class FeedForwardMx8(Function):
         return (dh @ w1 if ctx.needs_input_grad[0] else None), dW1, db1, dW2, db2, None, None, None
 
 
-def _mx8_linear(lin: torch.nn.Linear) -> bool:
+def mx8_linear(lin: torch.nn.Linear) -> bool:
+    """Whether the backward of `lin` can take its input in 8 bits (under autograd)."""
     return (lin.in_features, lin.out_features) in mx8.WGRAD_SHAPES and lin.bias is not None and torch.is_grad_enabled()
 
 
 def feed_forward(lin1: torch.nn.Linear, lin2: torch.nn.Linear, x: torch.Tensor, act, checkpoint: str = 'none') -> torch.Tensor:
     """lin2(dropout_p(relu(lin1(x)))) per pair, act = (seed, salt, p); checkpoint='mx8' (where both Linears are built for it): the backward
     gets x and the hidden tensor in 8 bits."""
-    if checkpoint == 'mx8' and _mx8_linear(lin1) and _mx8_linear(lin2):
+    if checkpoint == 'mx8' and mx8_linear(lin1) and mx8_linear(lin2):
         return FeedForwardMx8.apply(x, lin1.weight, lin1.bias, lin2.weight, lin2.bias, *act)
     return wide_linear(lin2, wide_linear(lin1, x, act=act))
 
@@ -193,7 +194,7 @@ def wide_linear(lin: torch.nn.Linear, x: torch.Tensor, act=None, held: Optional[
     the GEMM's result (csrc/k_train_fused.hip).  `held` = mx8.quantize(x): the backward gets x in this 8-bit form (where
     da_linear_wgrad_mx8 is built for the shape)."""
     shape = (lin.in_features, lin.out_features)
-    if held is not None and act is None and _mx8_linear(lin):
+    if held is not None and act is None and mx8_linear(lin):
         return WideLinearMx8.apply(x, lin.weight, lin.bias, *held)
     if x.dtype == torch.bfloat16:
         if shape in _WGRAD_SHAPES and lin.bias is not None and torch.is_grad_enabled():
@@ -291,7 +292,7 @@ class HeadAttnCore(Function):
             # (the tensors behind the addresses are locals until the call returns)
             ctx.save_for_backward(Q, K, V, nm_u8, wV, st, *((codes, scales) if mx else (E1,)))
             ctx.meta = (n_head, qscale, cap, mx)
-        L.check(L.lib().da_attn_head_fwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), E1.data_ptr(), E2.data_ptr(), E1.dtype is torch.bfloat16,
+        L.raise_on(L.lib().da_attn_head_fwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), E1.data_ptr(), E2.data_ptr(), E1.dtype is torch.bfloat16,
                                          nm_u8.data_ptr(), 0 if groups is None else groups.data_ptr(), qscale, cap, Y.data_ptr(), wV.data_ptr(), sp, tp,
                                          cp, kp, B, n, dx, n_head, L.stream()), 'da_attn_head_fwd')
         return Y, wV
@@ -313,7 +314,7 @@ class HeadAttnCore(Function):
         # the workspace is this call's own: two captured graphs that are replayed side by side must not share one
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
         e1, tp = E1.data_ptr(), st.data_ptr()
-        L.check(lib.da_attn_head_bwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), 0 if mx else e1, e1 if mx else 0, scales[0].data_ptr() if mx else 0,
+        L.raise_on(lib.da_attn_head_bwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), 0 if mx else e1, e1 if mx else 0, scales[0].data_ptr() if mx else 0,
                                      nm_u8.data_ptr(), qscale, cap, wV.data_ptr(), tp + 8 * B * n * n_head, tp, dY.data_ptr(), dY.dtype is torch.bfloat16,
                                      dwV.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dE1.data_ptr(), dE2.data_ptr(), ws.data_ptr(), nbytes,
                                      B, n, dx, n_head, L.stream()), 'da_attn_head_bwd')
@@ -333,8 +334,8 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
       S = sum of Y over a head's channels, cap tanh(S / cap) with cap > 0;  wV = softmax_j(S) V
 
     E1 and E2 are not looked at where a node of the pair is masked.  The softmax runs over all keys, as in the reference, or with `groups`
-    (B,n) integers over the keys of the query's own group (a node with a negative group is in none: its wV is 0, and so is the wV of
-    every row without a key).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
+    (B,n) integers below 2^31 over the keys of the query's own group (a node with a negative group is in none: its wV is 0, and so is the
+    wV of every row without a key; V of keys outside the group is not looked at).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
     fp32 arithmetic throughout; sums do not depend on timing."""
     shape = Q.shape
     if len(shape) != 3 or K.shape != shape or V.shape != shape:
@@ -355,8 +356,8 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
     if checkpoint == 'mx8' and dx % mx8.GROUP:
         raise L.DiffAlignHipError(f"head_attention: checkpoint='mx8' needs dx % {mx8.GROUP} == 0, dx = {dx}")
     cap = float(cap)
-    if not 0.0 <= cap < math.inf:
-        raise ValueError(f'head_attention: cap = {cap}')
+    if not (cap == 0.0 or 1e-30 <= cap <= 1e30):
+        raise ValueError(f'head_attention: cap = {cap}: 0 (none) or in [1e-30, 1e30]')
     mx8.refuse_cpu(Q)
     if mx8.elsewhere(Q):
         with torch.cuda.device(dev):

@@ -545,7 +545,7 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
   DA_CHECK_ARG((S == nullptr) == (stat == nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr) && (!E1_codes || S),
                "da_attn_head_fwd: S and stat go together, E1's codes and scales with both");
   DA_CHECK_ARG(!E1_codes || dx % MX8_GROUP == 0, "da_attn_head_fwd: 8-bit E1 needs dx %% 32 == 0, dx = %d", dx);
-  DA_CHECK_ARG(cap >= 0.f && cap < INFINITY, "da_attn_head_fwd: cap = %g", cap);
+  DA_CHECK_ARG(cap == 0.f || (cap >= 1e-30f && cap <= 1e30f), "da_attn_head_fwd: cap = %g: 0 (none) or in [1e-30, 1e30]", cap);
   DA_CHECK_ARG(al16({Q, K, V, E1, E2, Y, wV, E1_codes}) && ((uintptr_t)stat & 7) == 0 && ((uintptr_t)S & 3) == 0, "da_attn_head_fwd: unaligned tensor (16 bytes)");
   a.Q = Q; a.K = K; a.V = V; a.E1 = E1; a.E2 = E2; a.nm = node_mask; a.grp = groups; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx; a.H = n_head;
   a.Y = Y; a.wV = wV; a.S = S; a.stat = stat; a.q1 = (uint8_t*)E1_codes; a.q1s = E1_scales; a.B = B;
@@ -576,7 +576,7 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
   DA_CHECK_ARG((E1 != nullptr) != (E1_codes != nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr),
                "da_attn_head_bwd: E1 either at full width or as codes and scales");
   DA_CHECK_ARG(!E1_codes || dx % MX8_GROUP == 0, "da_attn_head_bwd: 8-bit E1 needs dx %% 32 == 0, dx = %d", dx);
-  DA_CHECK_ARG(cap >= 0.f && cap < INFINITY, "da_attn_head_bwd: cap = %g", cap);
+  DA_CHECK_ARG(cap == 0.f || (cap >= 1e-30f && cap <= 1e30f), "da_attn_head_bwd: cap = %g: 0 (none) or in [1e-30, 1e30]", cap);
   DA_CHECK_ARG(al16({Q, K, V, E1, E1_codes, wV, dY, dwV, dQ, dK, dV, dE1, dE2, workspace}) && ((uintptr_t)stat & 7) == 0 && ((uintptr_t)S & 3) == 0,
                "da_attn_head_bwd: unaligned tensor (16 bytes)");
   const long long need = da_attn_head_bwd_workspace(B, n, dx, n_head, dy_bf16);

@@ -39,8 +39,8 @@ class NodeEdgeBlock(nn.Module):
         self.improved = improved
         if scope not in ATTN_SCOPES:
             raise ValueError(f'attention scope {scope!r}: one of {ATTN_SCOPES}')
-        if not 0.0 <= float(score_cap) < float('inf'):
-            raise ValueError(f'score_cap = {score_cap}')
+        if not (score_cap == 0.0 or 1e-30 <= float(score_cap) <= 1e30):
+            raise ValueError(f'score_cap = {score_cap}: 0 (none) or in [1e-30, 1e30]')
         if not improved and (scope != 'all' or score_cap):
             raise ValueError('score_cap and scope belong to the per-head attention: improved=True')
         self.score_cap, self.scope = float(score_cap), scope

@@ -77,7 +77,7 @@ def quantize(x: torch.Tensor, keep_nonzero: bool = False) -> Mx8:
     D = shape[-1]
     codes = torch.empty(shape, dtype=torch.int8, device=x.device)
     scales = torch.empty(shape[:-1] + (-(-D // GROUP),), dtype=torch.uint8, device=x.device)
-    L.check(L.lib().da_mx8_quant(x.data_ptr(), x.dtype is torch.bfloat16, codes.data_ptr(), scales.data_ptr(), x.numel() // D, D, keep_nonzero, L.stream()),
+    L.raise_on(L.lib().da_mx8_quant(x.data_ptr(), x.dtype is torch.bfloat16, codes.data_ptr(), scales.data_ptr(), x.numel() // D, D, keep_nonzero, L.stream()),
             'da_mx8_quant')
     return Mx8(codes, scales)
 
@@ -94,7 +94,7 @@ def dequantize(q: Mx8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     if D == 0:
         return out
-    L.check(L.lib().da_mx8_dequant(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dtype is torch.bfloat16, out.numel() // D, D, L.stream()),
+    L.raise_on(L.lib().da_mx8_dequant(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dtype is torch.bfloat16, out.numel() // D, D, L.stream()),
             'da_mx8_dequant')
     return out
 
@@ -121,7 +121,7 @@ def linear_wgrad(q: Mx8, dy: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     lib = L.lib()
     nbytes = lib.da_linear_wgrad_mx8_workspace(R, in_f, out_f)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    L.check(lib.da_linear_wgrad_mx8(codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dy.dtype is torch.bfloat16, dW.data_ptr(), db.data_ptr(),
+    L.raise_on(lib.da_linear_wgrad_mx8(codes.data_ptr(), scales.data_ptr(), dy.data_ptr(), dy.dtype is torch.bfloat16, dW.data_ptr(), db.data_ptr(),
                                     ws.data_ptr(), nbytes, R, in_f, out_f, L.stream()), 'da_linear_wgrad_mx8')
     return dW, db
 
@@ -137,6 +137,6 @@ def relu_dropout_bwd(q: Mx8, dy: torch.Tensor, p: float) -> torch.Tensor:
             return relu_dropout_bwd(q, dy, p)
     dy = dy.contiguous()
     dx = torch.empty_like(dy)
-    L.check(L.lib().da_relu_dropout_bwd_mx8(codes.data_ptr(), dy.data_ptr(), dx.data_ptr(), dy.dtype is torch.bfloat16, dy.numel(), float(p), L.stream()),
+    L.raise_on(L.lib().da_relu_dropout_bwd_mx8(codes.data_ptr(), dy.data_ptr(), dx.data_ptr(), dy.dtype is torch.bfloat16, dy.numel(), float(p), L.stream()),
             'da_relu_dropout_bwd_mx8')
     return dx

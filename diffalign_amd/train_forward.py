@@ -21,7 +21,7 @@ import torch.nn.functional as F
 from . import _lib as L
 from . import mx8
 from .autograd_ops import (AttnCore, AttnCoreBF16, AddLayerNorm, PoolStats, MaskDense, ResidualLN, ReluDropout, FUSED_WIDTHS, qscale_of,
-                           wide_linear, feed_forward, head_attention, head_attention_built)
+                           wide_linear, feed_forward, head_attention, head_attention_built, mx8_linear)
 
 
 # The node (B n rows) and y (B rows) sides of a layer are ~150 launches of a few microseconds each, forward plus backward, beside a
@@ -68,9 +68,9 @@ class _Lanes:
         return ts
 
 
-def _hold(x, checkpoint):
-    """x in 8 bits for the backward pass (checkpoint == 'mx8' under autograd), else None."""
-    return mx8.quantize(x) if checkpoint == 'mx8' and torch.is_grad_enabled() else None
+def _hold(x, lin, checkpoint):
+    """x, the input of `lin`, in 8 bits for the backward pass (checkpoint == 'mx8', where built), else None."""
+    return mx8.quantize(x) if checkpoint == 'mx8' and mx8_linear(lin) else None
 
 
 def _node_edge_block(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False, checkpoint='none'):
@@ -84,12 +84,12 @@ def _node_edge_block(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fused=False
     pE = PoolStats.apply(E)
     bf = Eb is not None and a.dx % 4 == 0 and 256 % (a.dx // 4) == 0
     src = Eb if bf else E
-    held = _hold(src, checkpoint)
+    held = _hold(src, a.e_mul, checkpoint)
     E1, E2 = wide_linear(a.e_mul, src, held=held), wide_linear(a.e_add, src, held=held)
     lanes.to_pair(Q, K, V, yea, yem)
     Z, wV = (AttnCoreBF16 if bf else AttnCore).apply(Q, K, V, E1, E2, nm_u8, yea, yem, qscale_of(a.dx, a.n_head))
     lanes.to_node(wV, pE)
-    newE = wide_linear(a.e_out, Z, held=_hold(Z, checkpoint))
+    newE = wide_linear(a.e_out, Z, held=_hold(Z, a.e_out, checkpoint))
     if not fused:                     # fused: the mask (and the widening) happen inside the residual block's kernel
         newE = (newE.float() if bf else newE) * em
     with lanes.on_node():
@@ -108,7 +108,7 @@ def _node_edge_block_improved(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fu
         pX = PoolStats.apply(X)
     pE = PoolStats.apply(E)
     src = E if Eb is None else Eb
-    held = _hold(src, checkpoint)
+    held = _hold(src, a.e_mul, checkpoint)
     E1, E2 = wide_linear(a.e_mul, src, held=held), wide_linear(a.e_add, src, held=held)       # :115-122
     lanes.to_pair(Q, K, V)
     if head_attention_built(a.dx, a.n_head):
@@ -117,7 +117,7 @@ def _node_edge_block_improved(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fu
     else:
         Y, wV = _head_attention_torch(a, Q, K, V, E1, E2, em, groups)
     lanes.to_node(wV, pE)
-    newE = wide_linear(a.e_out, Y, held=_hold(Y, checkpoint))                                 # :123-125
+    newE = wide_linear(a.e_out, Y, held=_hold(Y, a.e_out, checkpoint))                                 # :123-125
     if not fused:
         newE = newE.float() * em
     with lanes.on_node():

@@ -195,7 +195,7 @@ int da_relu_dropout(void* h, int is_bf16, long long numel, const long long* seed
 int da_relu_dropout_bwd(const void* h, const void* dy, void* dx, int is_bf16, long long numel, float p, void* stream);
 /* ---- per-head edge attention (NodeEdgeBlockImproved, neuralnet/layers.py:115-141), forward and backward.  m_ij = m_i m_j:
  *   Y = qscale Q_i K_j (1 + m_ij E1) + m_ij E2 (the input of e_out);  S = sum of Y over a head's dx / n_head channels, cap tanh(S / cap) with
- *   cap > 0;  wV = softmax over keys of S times V.  groups (B,n) int32 (NULL: all keys, as the reference): row i sees the keys with
+ *   cap in [1e-30, 1e30] (0: none);  wV = softmax over keys of S times V.  groups (B,n) int32 (NULL: all keys, as the reference): row i sees the keys with
  *   groups[j] == groups[i] >= 0; a row without a key gets wV = 0.  E1 and E2 are not read where m_ij = 0.
  * Q, K, V, wV (B,n,dx) fp32; E1, E2, Y (B,n,n,dx) fp32 or bf16 (e_bf16).  For a backward: S (B,n,n,n_head) fp32 and stat (B,n,n_head,2) are
  * written when given (both or neither), and E1_codes / E1_scales get E1 in 8 bits (da_mx8_quant's format; dx % 32 == 0).

@@ -43,7 +43,7 @@ def test_refusals():
         with pytest.raises(L.DiffAlignHipError):                            # (the first: CPU tensors)
             head_attention(**{**ok(), **bad})
         L._held.clear()
-    for bad in (dict(cap=-1.0), dict(cap=float('nan')), dict(cap=float('inf')), dict(checkpoint='8bit')):
+    for bad in (dict(cap=-1.0), dict(cap=float('nan')), dict(cap=float('inf')), dict(cap=1e-38), dict(cap=1e38), dict(checkpoint='8bit')):
         with pytest.raises(ValueError):
             head_attention(**{**ok(), **bad})
     with pytest.raises(L.DiffAlignHipError):
@@ -60,7 +60,7 @@ def test_c_entries_refuse_before_any_launch():
     assert fwd(B=-1) == -1 and fwd(H=5) == -3 and fwd(dx=60, H=2) == -3 and fwd(dx=1024, H=32) == -3 and fwd(dx=512, H=128) == -3
     assert fwd(B=0) == 0 and fwd(n=0) == 0
     assert fwd(Q=0) == -1 and fwd(S=p) == -1 and fwd(c=p, sc=p) == -1 and fwd(S=p, st=p, c=p) == -1
-    assert fwd(cap=-1.0) == -1 and fwd(cap=float('nan')) == -1 and fwd(E1=24) == -1 and b'unaligned' in lib.da_last_error()
+    assert fwd(cap=-1.0) == -1 and fwd(cap=float('nan')) == -1 and fwd(cap=1e-38) == -1 and fwd(cap=1e38) == -1 and fwd(E1=24) == -1 and b'unaligned' in lib.da_last_error()
     assert fwd(n=1 << 22) == -1 and b'too large' in lib.da_last_error()
     assert fwd(S=p, st=p, c=p, sc=p, dx=40, H=5) == -1 and b'32' in lib.da_last_error()
     bwd = lambda **k: lib.da_attn_head_bwd(*[{**dict(Q=p, K=p, V=p, E1=p, c=0, sc=0, nm=p, qs=1.0, cap=0.0, wV=p, S=p, st=p, dY=p, bf=0, g=p, dQ=p, dK=p, dV=p, d1=p,
