@@ -19,6 +19,13 @@ def _c(t):
     return t.contiguous().float()
 
 
+def _once(backward):
+    """A backward that is differentiable once: under create_graph (autograd then runs it with gradients on) what it returns refuses to be
+    differentiated again; otherwise it is called as it is."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 def _c16(t):
     """contiguous fp32 at a 16-byte aligned address (kernels that read float4)."""
     t = _c(t)
@@ -124,7 +131,7 @@ class WideLinearMx8(Function):
         return torch.nn.functional.linear(x, w, b)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         codes, scales, w = ctx.saved_tensors
         dy = dy.contiguous()
@@ -148,7 +155,7 @@ class FeedForwardMx8(Function):
         return torch.nn.functional.linear(h, w2, b2)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         codes, scales, hc, hs, w1, w2 = ctx.saved_tensors
         dy = dy.contiguous()
@@ -298,7 +305,7 @@ class HeadAttnCore(Function):
         return Y, wV
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dY, dwV):
         Q, K, V, nm_u8, wV, st, E1, *scales = ctx.saved_tensors
         if mx8.elsewhere(Q):
@@ -307,15 +314,16 @@ class HeadAttnCore(Function):
         n_head, qscale, cap, mx = ctx.meta
         B, n, dx = Q.shape
         dY, dwV = mx8.aligned(dY), mx8.aligned(dwV)
+        bf16 = dY.dtype is torch.bfloat16
         dQ, dK, dV = torch.empty_like(Q), torch.empty_like(Q), torch.empty_like(Q)
         dE1, dE2 = torch.empty_like(dY), torch.empty_like(dY)
         lib = L.lib()
-        nbytes = lib.da_attn_head_bwd_workspace(B, n, dx, n_head, dY.dtype is torch.bfloat16)
+        nbytes = lib.da_attn_head_bwd_workspace(B, n, dx, n_head, bf16)
         # the workspace is this call's own: two captured graphs that are replayed side by side must not share one
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
         e1, tp = E1.data_ptr(), st.data_ptr()
         L.raise_on(lib.da_attn_head_bwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), 0 if mx else e1, e1 if mx else 0, scales[0].data_ptr() if mx else 0,
-                                     nm_u8.data_ptr(), qscale, cap, wV.data_ptr(), tp + 8 * B * n * n_head, tp, dY.data_ptr(), dY.dtype is torch.bfloat16,
+                                     nm_u8.data_ptr(), qscale, cap, wV.data_ptr(), tp + 8 * B * n * n_head, tp, dY.data_ptr(), bf16,
                                      dwV.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dE1.data_ptr(), dE2.data_ptr(), ws.data_ptr(), nbytes,
                                      B, n, dx, n_head, L.stream()), 'da_attn_head_bwd')
         return dQ, dK, dV, dE1, dE2, None, None, None, None, None, None, None

@@ -233,3 +233,16 @@ def test_offsets_past_32_bits():
             assert torch.equal(a, b)
         else:
             assert bool((a - b).norm() <= (2.0 ** -7 if name in ('dE1', 'dE2') else 1e-3) * b.norm()), (name, float((a - b).norm() / b.norm()))
+
+
+def test_second_derivative_is_refused():
+    """Differentiable once: under create_graph the gradients come out as ever, and refuse to be differentiated again."""
+    from diffalign_amd.autograd_ops import head_attention
+    t, nm, gr, dY, dwV = inputs(1, 7, 64, torch.float32, 4, False)
+    want = run(t, nm, None, dY, dwV, 4, 0.0, 'none')
+    leaves = [x.to(D_).requires_grad_(True) for x in t]
+    Y, wV = head_attention(*leaves, nm.to(D_), 4)
+    grads = torch.autograd.grad((Y, wV), leaves, (dY.to(D_), dwV.to(D_)), create_graph=True)
+    assert all(torch.equal(a.detach(), b) for a, b in zip(grads, want[2:]))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(grads[0].sum(), leaves[3])
