@@ -19,20 +19,26 @@ __device__ __forceinline__ unsigned mx8_scale(unsigned amax_bits) {
 __device__ __forceinline__ float mx8_inv(unsigned b) { return __builtin_bit_cast(float, b == 255u ? 0u : (260u - b) << 23); }
 // X / 64: what a code stands for
 __device__ __forceinline__ float mx8_step(unsigned b) { return __builtin_bit_cast(float, b == 255u ? 0x7fc00000u : (b - 6u) << 23); }
-// round to nearest even of x * inv, as the low byte of a word: 1.5 * 2^23 has a unit of 1, and x * inv is exact (a power of two) unless it
-// is far below one half.  The clamp acts only where the scale is saturated (or x is not finite: that group's codes are 0).
+// round to nearest even of x * inv in the low byte of a word: 1.5 * 2^23 has a unit of 1 and x * inv is exact (a power of two) unless it is
+// far below one half, so the fused sum rounds once.  The clamp acts only where the scale is saturated (or x is not finite: inv = 0, and
+// that group's codes are 0).
+__device__ __forceinline__ unsigned mx8_round(float x, float inv) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_fmed3f(__builtin_fmaf(x, inv, 12582912.f), 12582912.f - 127.f, 12582912.f + 127.f));
+}
 // KEEP: an element other than zero never gets code 0 (+-1 instead), so the codes still tell what a ReLU let through.
 template <bool KEEP>
 __device__ __forceinline__ unsigned mx8_code(float x, float inv) {
-  const float t = __builtin_amdgcn_fmed3f(x * inv, -127.f, 127.f) + 12582912.f;
-  unsigned w = inv == 0.f ? 0u : __builtin_bit_cast(unsigned, t) & 0xffu;
+  unsigned w = inv == 0.f ? 0u : mx8_round(x, inv) & 0xffu;
   if (KEEP && w == 0u && x != 0.f) w = x > 0.f ? 1u : 0xffu;
   return w;
 }
 // four codes (element order) in one word
 template <bool KEEP>
 __device__ __forceinline__ unsigned mx8_pack4(float a, float b, float c, float d, float inv) {
-  return mx8_code<KEEP>(a, inv) | mx8_code<KEEP>(b, inv) << 8 | mx8_code<KEEP>(c, inv) << 16 | mx8_code<KEEP>(d, inv) << 24;
+  if constexpr (KEEP) return mx8_code<true>(a, inv) | mx8_code<true>(b, inv) << 8 | mx8_code<true>(c, inv) << 16 | mx8_code<true>(d, inv) << 24;
+  const unsigned ab = __builtin_amdgcn_perm(mx8_round(b, inv), mx8_round(a, inv), 0x0c0c0400u);
+  const unsigned cd = __builtin_amdgcn_perm(mx8_round(d, inv), mx8_round(c, inv), 0x0c0c0400u);
+  return inv == 0.f ? 0u : __builtin_amdgcn_perm(cd, ab, 0x05040100u);
 }
 // signed byte k of a word as a float
 template <int K>
