@@ -343,7 +343,7 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
 
     E1 and E2 are not looked at where a node of the pair is masked.  The softmax runs over all keys, as in the reference, or with `groups`
     (B,n) integers below 2^31 over the keys of the query's own group (a node with a negative group is in none: its wV is 0, and so is the
-    wV of every row without a key; V of keys outside the group is not looked at).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
+    wV of every row without a key; V of keys outside the group, or with a score of -inf, has no effect).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
     fp32 arithmetic throughout; sums do not depend on timing."""
     shape = Q.shape
     if len(shape) != 3 or K.shape != shape or V.shape != shape:

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(256) k_attn_head_fwd(HeadArgs a) {
       }
       s = head_sum<HLOG>(s);
       if (a.cap > 0.f) s = a.cap * tanhf(s * inv_cap);
-      const bool on = gj >= 0 && gj == gi[t];
+      const bool on = (gj >= 0) & (gj == gi[t]) & (s != -INFINITY);      // (a score of -inf shuts the key out like a group does: V is not looked at)
       s = on ? s : -INFINITY;
       if constexpr (SAVE)
         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, s), rS, oS + t * (unsigned)(n * H) * 4, 0, 0);

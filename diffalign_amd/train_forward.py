@@ -110,6 +110,8 @@ def _node_edge_block_improved(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fu
     src = E if Eb is None else Eb
     held = _hold(src, a.e_mul, checkpoint)
     E1, E2 = wide_linear(a.e_mul, src, held=held), wide_linear(a.e_add, src, held=held)       # :115-122
+    if E1.dtype not in (torch.float32, torch.bfloat16):                                        # (fp16 under a caller's autocast)
+        E1, E2 = E1.float(), E2.float()
     lanes.to_pair(Q, K, V)
     if head_attention_built(a.dx, a.n_head):
         Y, wV = head_attention(Q, K, V, E1, E2, nm_u8, a.n_head, cap=a.score_cap, groups=groups,
@@ -151,6 +153,8 @@ def _attn_groups(m, node_mask, mol_assignments):
     if scope == 'all':
         return None
     side = torch.zeros_like(node_mask, dtype=torch.int32)
+    if scope == 'side' and mol_assignments is None:
+        raise ValueError("attn_scope='side' needs mol_assignments")
     if scope == 'side':       # 1 = product (the molecule with the largest number, as in align_index), 0 = reactants
         side = (mol_assignments == mol_assignments.max(-1, keepdim=True).values).int()
     return torch.where(node_mask.bool(), side, -1).int()

@@ -196,7 +196,8 @@ int da_relu_dropout_bwd(const void* h, const void* dy, void* dx, int is_bf16, lo
 /* ---- per-head edge attention (NodeEdgeBlockImproved, neuralnet/layers.py:115-141), forward and backward.  m_ij = m_i m_j:
  *   Y = qscale Q_i K_j (1 + m_ij E1) + m_ij E2 (the input of e_out);  S = sum of Y over a head's dx / n_head channels, cap tanh(S / cap) with
  *   cap in [1e-30, 1e30] (0: none);  wV = softmax over keys of S times V.  groups (B,n) int32 (NULL: all keys, as the reference): row i sees the keys with
- *   groups[j] == groups[i] >= 0; a row without a key gets wV = 0.  E1 and E2 are not read where m_ij = 0.
+ *   groups[j] == groups[i] >= 0; a row without a key gets wV = 0.  E1 and E2 are not read where m_ij = 0, V of a key
+ *   outside the group or with a score of -inf has no effect.
  * Q, K, V, wV (B,n,dx) fp32; E1, E2, Y (B,n,n,dx) fp32 or bf16 (e_bf16).  For a backward: S (B,n,n,n_head) fp32 and stat (B,n,n_head,2) are
  * written when given (both or neither), and E1_codes / E1_scales get E1 in 8 bits (da_mx8_quant's format; dx % 32 == 0).
  * Built: 4, 8, 16, .. 128 channels per head, dx <= 512 (256 with 4 channels per head); others: DA_ERR_UNSUPPORTED.  Tensors 16-byte aligned (stat 8,
@@ -214,8 +215,8 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
                      long long workspace_bytes, int B, int n, int dx, int n_head, void* stream);
 /* ---- 8-bit activation checkpoints of the training step (the reference keeps full-width activations for loss.backward(),
  * training/helpers.py:139-142).  MXINT8: 32 consecutive channels of a row share the scale 2^(b-127) (one byte b), an element is an int8 q and
- * stands for q / 64 * 2^(b-127); b is the smallest in [27, 254] at which the group's largest magnitude rounds to 127 or less, 255 (codes 0: the
- * group stands for NaN) where the group holds an infinity or NaN.  codes (rows, D), scales (rows, ceil(D / 32)). ---- */
+ * stands for q / 64 * 2^(b-127); b is the smallest in [27, 254] at which the group's largest magnitude rounds to 127 or less, 255 (the
+ * group stands for NaN, whatever its codes) where the group holds an infinity or NaN.  codes (rows, D), scales (rows, ceil(D / 32)). ---- */
 
 /* Quantise x (rows, D) fp32 or bf16 (x_bf16).  keep_nonzero: an element other than zero gets a code other than zero.  Any D >= 1; D % 32
  * == 0 with x 16-byte and codes 8-byte aligned takes the wide path. */

@@ -112,6 +112,9 @@ def test_bias_of_lowest_value_and_minus_infinity():
             t[4][0, 2] = shut                                               # row 2 sees nothing
             dY[0, :, 4] = 0; dY[0, 2] = 0
             got = run(t, nm, None, dY, dwV, 4, 0.0, 'none')
+            nan = [x.clone() for x in t]
+            nan[2][0, 4] = float('nan')                                     # what a shut key's V holds has no effect
+            assert all(torch.equal(a, b) for a, b in zip(run(nan, nm, None, dY, dwV, 4, 0.0, 'none'), got))
             assert (got[1][0, 2] == 0).all() and torch.isfinite(got[1]).all()
             assert all(torch.isfinite(x).all() for x in got[2:]) and (got[4][0, 4] == 0).all()
             keep = [j for j in range(9) if j != 4]

@@ -127,3 +127,60 @@ def test_linear_wgrad_many_rows_and_nonfinite():
     ok = torch.ones(o, dtype=torch.bool); ok[3] = ok[7] = False
     assert torch.isfinite(dW.cpu()[ok]).all() and torch.isfinite(db.cpu()[ok]).all()
     assert torch.isinf(db[3]) and torch.isnan(db[7]) and torch.isnan(dW[7]).all() and not torch.isfinite(dW[3]).any()
+
+
+def test_offsets_past_32_bits():
+    """2.1e9 elements: the last rows of a large tensor through every kernel equal the same rows alone."""
+    from diffalign_amd import mx8
+    R, D = (1 << 23) + 5, 256
+    x = torch.zeros(R, D, dtype=torch.bfloat16, device=D_)
+    tail = act(9, D, torch.bfloat16, 1).to(D_)
+    x[-9:] = tail
+    q = mx8.quantize(x)
+    one = mx8.quantize(tail)
+    assert torch.equal(q.codes[-9:], one.codes) and torch.equal(q.scales[-9:], one.scales) and int(q.scales[:-9].max()) == 27
+    del x
+    assert torch.equal(mx8.dequantize(q, torch.bfloat16)[-9:], mx8.dequantize(one, torch.bfloat16))
+    dy = torch.zeros(R, 64, dtype=torch.bfloat16, device=D_)
+    dt = act(9, 64, torch.bfloat16, 2).to(D_)
+    dy[-9:] = dt
+    got, want = mx8.linear_wgrad(q, dy), mx8.linear_wgrad(one, dt)
+    # nine rows in one 16-row step of the matrix instruction, or in two: the same nine products in another order
+    S = dt.double().abs().t() @ mx8.dequantize(one).double().abs()
+    assert bool(((got[0] - want[0]).abs().double() <= 16 * 2.0 ** -23 * S).all())
+    h = mx8.relu_dropout_bwd(mx8.Mx8(q.codes[:, :64].contiguous(), q.scales[:, :2].contiguous()), dy, 0.0)
+    assert torch.equal(h[-9:], torch.where(one.codes[:, :64] != 0, dt, torch.zeros_like(dt)))
+
+
+def test_other_stream_and_captured_graphs():
+    """Two captured passes (quantise, weight gradient, restore) replayed in turn and side by side, with eager work between."""
+    from diffalign_amd import mx8
+    sets = []
+    for seed in (1, 2):
+        x, dy = act(3000, 64, torch.bfloat16, seed).to(D_), act(3000, 128, torch.bfloat16, seed + 5).to(D_)
+
+        def step(x, dy):
+            q = mx8.quantize(x)
+            return (mx8.dequantize(q),) + mx8.linear_wgrad(q, dy)
+        want = step(x, dy)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = step(x, dy)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = step(x, dy)
+        sets.append((graph, out, want, s, x, dy))
+    for k in range(3):
+        for graph, out, *_ in sets:
+            for o in out: o.zero_()
+        torch.cuda.synchronize()
+        for graph, out, want, s, *_ in sets:
+            with torch.cuda.stream(s): graph.replay()
+        torch.cuda.synchronize()
+        for graph, out, want, *_ in sets:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        torch.randn(1 << 20, device=D_).sum()
+        torch.cuda.synchronize()
