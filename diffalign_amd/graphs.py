@@ -3,7 +3,10 @@ chain of small graphs (GraphedChain: one graph per step number, replayed for eve
 (GraphedTrainStep: the whole step, one graph per batch shape)."""
 from __future__ import annotations
 
+import gc
 import os
+import weakref
+from contextlib import contextmanager
 from typing import Optional
 from collections import OrderedDict
 
@@ -37,10 +40,25 @@ def _prepare_capture(dev) -> None:
         with torch.cuda.stream(s):
             x = torch.zeros(8, device=dev)
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
+            with _capture(g):
                 x += 1
         torch.cuda.current_stream(dev).wait_stream(s)
     _CAPTURE_READY.add(key)
+
+
+@contextmanager
+def _capture(graph, **kw):
+    """torch.cuda.graph with Python's cycle collector off: a captured body is thousands of Python allocations, and a collection among them
+    destroys whatever unreachable objects it finds -- other graphs, their memory pools, streams, events -- in the middle of the capture
+    (or on autograd's thread).  A destroyed graph's executable and pool must not go while another graph is being recorded."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, **kw):
+            yield
+    finally:
+        if on:
+            gc.enable()
 
 
 def chain_graphs_wanted(B: int, n: int) -> bool:
@@ -83,7 +101,7 @@ class GraphedTrainStep:
                 model.train_one_step(self.data, optimizer, group=group, pos_encodings=self.pos, update_ema=False)
         torch.cuda.current_stream().wait_stream(s)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with _capture(self.graph):
             self.loss = model.train_one_step(self.data, optimizer, group=group, pos_encodings=self.pos, update_ema=False)
         for b, k in zip(bufs, keep):                         # the capture pass enqueued nothing; the warm-up steps are taken back
             b.copy_(k)
@@ -117,7 +135,9 @@ class GraphedTrainStep:
         ready = torch.cuda.current_stream().record_event()      # next_data's tensors are ordered behind what the caller enqueued so far
         self.graph.replay()
         if self.pos is not None and next_data is not None and next_data is not self.data:
-            side = self.__dict__.setdefault('_pos_stream', torch.cuda.Stream())
+            side = self.__dict__.get('_pos_stream')
+            if side is None:                                     # (made once: torch hands streams out of a pool of 32, in turn)
+                side = self._pos_stream = torch.cuda.Stream()
             with torch.cuda.stream(side):
                 side.wait_event(ready)                           # (not for the replay: the encodings read next_data only)
                 pos_next = self.model.get_pos_encodings(next_data)
@@ -149,8 +169,11 @@ class GraphedChain:
         cache = model.__dict__.setdefault('_chain_graphs', OrderedDict())
         pm = model._net()._pack(data.X.device)
         if key in cache and cache[key].pm is not pm:
+            torch.cuda.synchronize(data.X.device)            # its last replays may still run
             del cache[key]                                   # the weights moved: the packed bf16 copies the graphs point at are stale
         if key not in cache:
+            if len(cache) >= CHAIN_GRAPH_CACHE:
+                torch.cuda.synchronize(data.X.device)
             while len(cache) >= CHAIN_GRAPH_CACHE:
                 cache.popitem(last=False)
             cache[key] = GraphedChain(model, data, masks, pos, temps, fix_nodes, fix_edges, with_eig_cache, first_call)
@@ -163,7 +186,10 @@ class GraphedChain:
         dev = data.X.device
         _prepare_capture(dev)
         B, n, kx = data.X.shape
-        self.model, self.temps, self.first_call, self.B, self.n = model, tuple(temps), int(first_call), B, n
+        # the model owns its chains; a strong reference back would be a cycle, and dropping the model would leave its graphs to Python's cycle
+        # collector, which destroys them wherever it happens to run
+        self._model = weakref.ref(model)
+        self.temps, self.first_call, self.B, self.n = tuple(temps), int(first_call), B, n
         self.pm = model._net()._pack(dev)                    # the packed weights the graphs point at (kept alive; identity = freshness)
         self.T_eval = int(model.cfg.diffusion.diffusion_steps_eval)
         cl = lambda t: None if t is None else t.clone()
@@ -197,6 +223,13 @@ class GraphedChain:
         self.graphs = {}
         self.pool = torch.cuda.graph_pool_handle()
         self.warm = False
+
+    @property
+    def model(self):
+        m = self._model()
+        if m is None:
+            raise RuntimeError('GraphedChain: its model, whose weights and tables the graphs read, is gone')
+        return m
 
     def load(self, data, masks, pos, fix_nodes, fix_edges, seeds, z_start, eig_cache, pad_noise, t_start=None):
         """A new chain of this shape: its inputs go into the static buffers, the eigensolver's cache starts empty.
@@ -264,6 +297,7 @@ class GraphedChain:
 
     def run_steps(self, t_from: int, t_to: int):
         """Steps t_from, t_from - 1, ..., t_to on the loaded chain (whose state sits in the input holder of step t_from)."""
+        model = self.model                                   # held for the length of the call
         with torch.no_grad():
             for t in range(t_from, t_to - 1, -1):
                 g = self.graphs.get(t)
@@ -281,7 +315,7 @@ class GraphedChain:
                             self.eig.state.copy_(keep)
                         self.warm = True
                     g = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(g, pool=self.pool):
+                    with _capture(g, pool=self.pool):
                         self._body(t)
                     self.graphs[t] = g
                 g.replay()
