@@ -20,6 +20,12 @@ from .placeholder import PlaceHolder
 # CHAIN_GRAPH_MAX_PAIRS pairs (B n^2) -- above, the edge kernels hide the host (B = 64, n = 300: 5.8 M pairs).  '0' / '1' force it.
 CHAIN_GRAPHS = os.environ.get('DA_CHAIN_GRAPHS', 'auto')
 CHAIN_GRAPH_MAX_PAIRS = 1_600_000
+# A step that computes the extra features (two batched library products and the eigensolver inside the capture, on top of the three streams) is
+# not captured: replaying such a chain ended the process inside the runtime's graph launch (a segmentation fault on the host, twice at the same
+# place in processes that had run 303 GPU tests before it, not in one that had run 196), while chains without them replayed in the same process.
+# No mistake on this side was found that accounts for it, so those chains run eagerly -- the same kernels, the same samples bit for bit --
+# also under DA_CHAIN_GRAPHS=1, and GraphedChain refuses them.
+CHAIN_GRAPH_EXTRA_FEATURES = False
 CHAIN_GRAPH_CACHE = 3            # shapes kept per model (each holds its graphs' private memory pool)
 
 
@@ -61,7 +67,10 @@ def _capture(graph, **kw):
             gc.enable()
 
 
-def chain_graphs_wanted(B: int, n: int) -> bool:
+def chain_graphs_wanted(B: int, n: int, extra_features: bool = False) -> bool:
+    """`extra_features`: the steps compute them (see CHAIN_GRAPH_EXTRA_FEATURES)."""
+    if extra_features and not CHAIN_GRAPH_EXTRA_FEATURES:
+        return False
     if CHAIN_GRAPHS == '0' or torch.cuda.is_current_stream_capturing():
         return False
     return CHAIN_GRAPHS == '1' or B * n * n <= CHAIN_GRAPH_MAX_PAIRS
@@ -153,7 +162,7 @@ class GraphedTrainStep:
 class GraphedChain:
     """The reverse chain of SamplingMixin.sample_one_batch for one batch shape, every step a HIP graph of the SAME work the eager loop
     enqueues: the fused reverse step with its three-stream arrangement (engine._layers_node_on_main: the side streams join the
-    capture through their events), the extra features with the eigensolver's fixed-block cache, the draw from per-chain counter
+    capture through their events), the draw from per-chain counter
     noise, apply_mask and inpainting.  One graph per step number t (the step's transition tables, its y input and its noise call index
     are constants of that graph), captured the first time the step runs and replayed for every later chain of the same shape; what a
     chain brings -- condition, masks, positional encodings, seeds, inpainting lists, start state -- is copied into static buffers.
@@ -181,8 +190,9 @@ class GraphedChain:
         return cache[key]
 
     def __init__(self, model, data, masks, pos, temps, fix_nodes, fix_edges, with_eig_cache, first_call):
-        from . import _lib as L
         from .extra_features import EigCache
+        if with_eig_cache and not CHAIN_GRAPH_EXTRA_FEATURES:
+            raise NotImplementedError('GraphedChain: steps that compute the extra features are not captured (CHAIN_GRAPH_EXTRA_FEATURES)')
         dev = data.X.device
         _prepare_capture(dev)
         B, n, kx = data.X.shape

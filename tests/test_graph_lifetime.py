@@ -108,3 +108,14 @@ def test_a_chain_without_its_model_refuses(chain):
     del model
     with pytest.raises(RuntimeError, match='model'):
         c.run()
+
+
+def test_extra_features_are_not_captured(chain, monkeypatch):
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    monkeypatch.setattr(graphs, 'CHAIN_GRAPHS', '1')
+    assert graphs.chain_graphs_wanted(5, 40) and not graphs.chain_graphs_wanted(5, 40, extra_features=True)
+    model = Model()
+    data = PlaceHolder(X=torch.zeros(B, N, KX), E=torch.zeros(B, N, N, KE), y=torch.zeros(B, 1), node_mask=torch.ones(B, N, dtype=torch.bool))
+    with pytest.raises(NotImplementedError, match='extra features'):
+        graphs.GraphedChain.get(model, data, (torch.ones(B, N, KX), torch.ones(B, N, N, KE)), None, (1.0, 1.0), None, None, True, 0)
+    assert len(model._chain_graphs) == 0
