@@ -408,7 +408,7 @@ def main():
         state['t'] = t - 1 if t > 1 else 50
 
     from diffalign_amd import graphs as G
-    use_graph = args.graph == 'on' or (args.graph == 'auto' and G.chain_graphs_wanted(B, n, args.extra_features == 'device'))
+    use_graph = args.graph == 'on' or (args.graph == 'auto' and G.chain_graphs_wanted(B, n))
     eager_step = step
     if use_graph:
         # as sample_one_batch does for a batch of this size: every step a HIP graph of the same fused, three-stream work; the steps the

@@ -23,7 +23,7 @@ ABI_VERSION = 4      # DA_ABI_VERSION of include/diffalign_hip.h this binding wa
 # (tests/test_abi_exports.py checks this table against the header).
 SIGNATURES = {
     'da_abi_version': 'i:',
-    'da_init': 'i:',
+    'da_init': 'i:', 'da_stream_create': 'i:p',
     'da_last_error': 's:',
     'da_mask_dense': 'i:pppiiiip',
     'da_collapse': 'i:pppppiiiip',

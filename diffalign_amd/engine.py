@@ -11,6 +11,7 @@ import torch
 
 from . import _lib as L
 from . import pack
+from . import streams
 
 N_STAT_CHUNKS = 32                    # most partial sums per graph of the separate Etoy statistics pass (stat_chunks)
 N_XSTAT_CHUNKS = 8
@@ -344,9 +345,6 @@ def layer_forward(pm: PackedModel, lw: dict, X, E_bf16, y, nm_u8, estats, B, n):
     return X2, E_out, layer_y(pm, lw, X, y, estats if estats is not None else tail, B, n)
 
 
-_SIDE = {}
-
-
 def _side_stream(dev):
     """Second HIP stream for the latency-bound tail of the y branch (none under HIP-graph capture).  The pooled statistics
     of a layer's input stay on the main stream (one HBM-bound pass; the edge kernel owns every CU's registers, nothing
@@ -357,10 +355,7 @@ def _side_stream(dev):
     stages, and (helpers.posterior_sample) the node half of the reverse step.  Returns (y stream, node stream) or None."""
     if torch.cuda.is_current_stream_capturing() and not CAPTURE_SIDE_STREAMS:
         return None
-    key = (dev.index if dev.index is not None else torch.cuda.current_device())
-    if key not in _SIDE:
-        _SIDE[key] = (torch.cuda.Stream(device=dev), torch.cuda.Stream(device=dev))
-    return _SIDE[key]
+    return streams.own(dev, 'y'), streams.own(dev, 'node')
 
 
 def _last_plan(last_rows):

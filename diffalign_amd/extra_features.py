@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
+from . import streams
 
 
 def _i(v):
@@ -79,7 +80,6 @@ class EigCache:
         return EigCache(torch.where(moving, idx, torch.zeros_like(idx)).amax(dim=1), n)
 
 
-_EIG_STREAMS = {}
 EIG_SIDE_STREAM = os.environ.get('DA_EIG_SIDE_STREAM', '1') != '0'      # A/B switch
 
 
@@ -87,10 +87,7 @@ def _eig_stream(dev):
     """Stream of the eigensolver beside the other feature kernels (none under HIP-graph capture)."""
     if not EIG_SIDE_STREAM or torch.cuda.is_current_stream_capturing():
         return None
-    key = dev.index if dev.index is not None else torch.cuda.current_device()
-    if key not in _EIG_STREAMS:
-        _EIG_STREAMS[key] = torch.cuda.Stream(device=dev)
-    return _EIG_STREAMS[key]
+    return streams.own(dev, 'eig')
 
 
 def _eigen(Lap: torch.Tensor, nm_u8: torch.Tensor, pad_noise: Optional[torch.Tensor], solver: Optional[str] = None,

@@ -12,7 +12,7 @@ from collections import OrderedDict
 
 import torch
 
-from . import helpers
+from . import helpers, streams
 from .placeholder import PlaceHolder
 
 # Reverse chains of SMALL graphs are host-bound: a step is ~130 kernel launches behind ~2 ms of Python / ctypes, while the GPU needs
@@ -20,12 +20,6 @@ from .placeholder import PlaceHolder
 # CHAIN_GRAPH_MAX_PAIRS pairs (B n^2) -- above, the edge kernels hide the host (B = 64, n = 300: 5.8 M pairs).  '0' / '1' force it.
 CHAIN_GRAPHS = os.environ.get('DA_CHAIN_GRAPHS', 'auto')
 CHAIN_GRAPH_MAX_PAIRS = 1_600_000
-# A step that computes the extra features (two batched library products and the eigensolver inside the capture, on top of the three streams) is
-# not captured: replaying such a chain ended the process inside the runtime's graph launch (a segmentation fault on the host, twice at the same
-# place in processes that had run 303 GPU tests before it, not in one that had run 196), while chains without them replayed in the same process.
-# No mistake on this side was found that accounts for it, so those chains run eagerly -- the same kernels, the same samples bit for bit --
-# also under DA_CHAIN_GRAPHS=1, and GraphedChain refuses them.
-CHAIN_GRAPH_EXTRA_FEATURES = False
 CHAIN_GRAPH_CACHE = 3            # shapes kept per model (each holds its graphs' private memory pool)
 
 
@@ -41,36 +35,28 @@ def _prepare_capture(dev) -> None:
     if key in _CAPTURE_READY or torch.cuda.is_current_stream_capturing():
         return
     with torch.inference_mode(False):
-        s = torch.cuda.Stream(device=dev)
-        s.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(s):
-            x = torch.zeros(8, device=dev)
-            g = torch.cuda.CUDAGraph()
-            with _capture(g):
-                x += 1
-        torch.cuda.current_stream(dev).wait_stream(s)
+        x = torch.zeros(8, device=dev)
+        with _capture(torch.cuda.CUDAGraph(), dev):
+            x += 1
     _CAPTURE_READY.add(key)
 
 
 @contextmanager
-def _capture(graph, **kw):
-    """torch.cuda.graph with Python's cycle collector off: a captured body is thousands of Python allocations, and a collection among them
-    destroys whatever unreachable objects it finds -- other graphs, their memory pools, streams, events -- in the middle of the capture
+def _capture(graph, dev, **kw):
+    """torch.cuda.graph on the framework's own capture stream (streams.own), with Python's cycle collector off: a captured body is thousands of
+    Python allocations, and a collection among them destroys whatever unreachable objects it finds -- other graphs, their memory pools, streams, events -- in the middle of the capture
     (or on autograd's thread).  A destroyed graph's executable and pool must not go while another graph is being recorded."""
     on = gc.isenabled()
     gc.disable()
     try:
-        with torch.cuda.graph(graph, **kw):
+        with torch.cuda.graph(graph, stream=streams.own(dev, 'capture'), **kw):
             yield
     finally:
         if on:
             gc.enable()
 
 
-def chain_graphs_wanted(B: int, n: int, extra_features: bool = False) -> bool:
-    """`extra_features`: the steps compute them (see CHAIN_GRAPH_EXTRA_FEATURES)."""
-    if extra_features and not CHAIN_GRAPH_EXTRA_FEATURES:
-        return False
+def chain_graphs_wanted(B: int, n: int) -> bool:
     if CHAIN_GRAPHS == '0' or torch.cuda.is_current_stream_capturing():
         return False
     return CHAIN_GRAPHS == '1' or B * n * n <= CHAIN_GRAPH_MAX_PAIRS
@@ -103,14 +89,14 @@ class GraphedTrainStep:
         bufs = [b for b in (opt.flat_param, opt.exp_avg, opt.exp_avg_sq, opt.max_exp_avg_sq, opt.step_dev) if b is not None]
         keep = [b.clone() for b in bufs]
         keep_host = (opt.steps, set(opt._ever), dict(opt._joined))
-        s = torch.cuda.Stream()
+        s = streams.own(example.X.device, 'warm')
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             for _ in range(warmup):                          # real steps on the example batch; undone below
                 model.train_one_step(self.data, optimizer, group=group, pos_encodings=self.pos, update_ema=False)
         torch.cuda.current_stream().wait_stream(s)
         self.graph = torch.cuda.CUDAGraph()
-        with _capture(self.graph):
+        with _capture(self.graph, example.X.device):
             self.loss = model.train_one_step(self.data, optimizer, group=group, pos_encodings=self.pos, update_ema=False)
         for b, k in zip(bufs, keep):                         # the capture pass enqueued nothing; the warm-up steps are taken back
             b.copy_(k)
@@ -144,9 +130,7 @@ class GraphedTrainStep:
         ready = torch.cuda.current_stream().record_event()      # next_data's tensors are ordered behind what the caller enqueued so far
         self.graph.replay()
         if self.pos is not None and next_data is not None and next_data is not self.data:
-            side = self.__dict__.get('_pos_stream')
-            if side is None:                                     # (made once: torch hands streams out of a pool of 32, in turn)
-                side = self._pos_stream = torch.cuda.Stream()
+            side = streams.own(self.data.X.device, 'pos')
             with torch.cuda.stream(side):
                 side.wait_event(ready)                           # (not for the replay: the encodings read next_data only)
                 pos_next = self.model.get_pos_encodings(next_data)
@@ -162,7 +146,7 @@ class GraphedTrainStep:
 class GraphedChain:
     """The reverse chain of SamplingMixin.sample_one_batch for one batch shape, every step a HIP graph of the SAME work the eager loop
     enqueues: the fused reverse step with its three-stream arrangement (engine._layers_node_on_main: the side streams join the
-    capture through their events), the draw from per-chain counter
+    capture through their events), the extra features with the eigensolver's fixed-block cache, the draw from per-chain counter
     noise, apply_mask and inpainting.  One graph per step number t (the step's transition tables, its y input and its noise call index
     are constants of that graph), captured the first time the step runs and replayed for every later chain of the same shape; what a
     chain brings -- condition, masks, positional encodings, seeds, inpainting lists, start state -- is copied into static buffers.
@@ -191,8 +175,6 @@ class GraphedChain:
 
     def __init__(self, model, data, masks, pos, temps, fix_nodes, fix_edges, with_eig_cache, first_call):
         from .extra_features import EigCache
-        if with_eig_cache and not CHAIN_GRAPH_EXTRA_FEATURES:
-            raise NotImplementedError('GraphedChain: steps that compute the extra features are not captured (CHAIN_GRAPH_EXTRA_FEATURES)')
         dev = data.X.device
         _prepare_capture(dev)
         B, n, kx = data.X.shape
@@ -316,7 +298,7 @@ class GraphedChain:
                         # one eager step on a side stream first (lazy set-up that must not happen under capture: weight packing,
                         # function attributes, allocator pools); the state it changes is put back
                         keep = None if self.eig is None else self.eig.state.clone()     # (the step's input holder is only read)
-                        s = torch.cuda.Stream()
+                        s = streams.own(self.seeds.device, 'warm')
                         s.wait_stream(torch.cuda.current_stream())
                         with torch.cuda.stream(s):
                             self._body(t)
@@ -325,7 +307,7 @@ class GraphedChain:
                             self.eig.state.copy_(keep)
                         self.warm = True
                     g = torch.cuda.CUDAGraph()
-                    with _capture(g, pool=self.pool):
+                    with _capture(g, self.seeds.device, pool=self.pool):
                         self._body(t)
                     self.graphs[t] = g
                 g.replay()

@@ -99,7 +99,7 @@ class SamplingMixin:
         recording = get_chains if record_chains is None else (get_chains and record_chains)
         from . import graphs
         if (not recording and not guided and chain_seeds is not None and self._net().supports_fused_step() and not self._net()._differentiable()
-                and graphs.chain_graphs_wanted(B, n, extra_features=eig_cache is not None)):
+                and graphs.chain_graphs_wanted(B, n)):
             gc = graphs.GraphedChain.get(self, dense_data, masks, pos_encodings, temps, fix_nodes, fix_edges, eig_cache is not None, calls[0])
             gc.load(dense_data, masks, pos_encodings, fix_nodes, fix_edges, chain_seeds, z_t, eig_cache, pad_noise)
             zg = gc.run()

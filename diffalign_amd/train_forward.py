@@ -19,7 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib as L
-from . import mx8
+from . import mx8, streams
 from .autograd_ops import (AttnCore, AttnCoreBF16, AddLayerNorm, PoolStats, MaskDense, ResidualLN, ReluDropout, FUSED_WIDTHS, qscale_of,
                            wide_linear, feed_forward, head_attention, head_attention_built, mx8_linear)
 
@@ -30,15 +30,6 @@ from .autograd_ops import (AttnCore, AttnCoreBF16, AddLayerNorm, PoolStats, Mask
 # so they run on a second stream; autograd replays every backward node on the stream of its forward, which gives the backward pass
 # the same overlap.  Tensors that cross are registered with the allocator (record_stream).  DA_TRAIN_SIDE_STREAM=0: one stream.
 SIDE_STREAM = _os.environ.get('DA_TRAIN_SIDE_STREAM', '1') != '0'
-_SIDE = {}
-
-
-def _side_stream(dev):
-    dev = torch.device(dev)
-    key = dev.index if dev.index is not None else torch.cuda.current_device()
-    if key not in _SIDE:
-        _SIDE[key] = torch.cuda.Stream(device=dev)
-    return _SIDE[key]
 
 
 class _Lanes:
@@ -46,7 +37,7 @@ class _Lanes:
 
     def __init__(self, dev, enabled):
         self.pair = torch.cuda.current_stream(dev)
-        self.node = _side_stream(dev) if enabled else self.pair
+        self.node = streams.own(dev, 'train_node') if enabled else self.pair
         self.split = self.node is not self.pair
 
     def on_node(self):

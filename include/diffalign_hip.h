@@ -26,6 +26,9 @@ const char* da_last_error(void);
 /* Per-device set-up that must not run under stream capture (today: the device address of da_edge_in_sym_static's scratch).  Call once
  * per device, with that device current, before the first captured call.  No counterpart in the reference. */
 int da_init(void);
+/* A stream of the current device at the default priority that does not wait for the null stream, for the caller to keep (*stream; it is not
+ * destroyed).  Not under stream capture.  No counterpart in the reference. */
+int da_stream_create(void** stream);
 
 /* ---- L0 container + masks ------------------------------------------------------------------------------------ */
 

@@ -2,13 +2,15 @@
 objects are replaced by recorders here, the class under test is graphs.GraphedChain itself."""
 import contextlib
 import gc
+import os
+import re
 import weakref
 from types import SimpleNamespace as ns
 
 import pytest
 import torch
 
-from diffalign_amd import graphs
+from diffalign_amd import graphs, streams
 from diffalign_amd.placeholder import PlaceHolder
 
 T_EVAL, B, N, KX, KE = 4, 2, 3, 5, 3
@@ -30,21 +32,45 @@ class Model:
 
 @pytest.fixture
 def chain(monkeypatch):
-    log = ns(collector=[], replays=0)
+    log = ns(collector=[], replays=0, ran=[], captured=[], on=[None])
+
+    class Stream:
+        def __init__(self, role):
+            self.role = role
+
+        def wait_stream(self, other):
+            pass
+
+    made = {}
+
+    @contextlib.contextmanager
+    def on(stream):
+        log.on.append(stream.role)
+        yield
+        log.on.pop()
+
+    def body(self, t):
+        log.collector.append(gc.isenabled())
+        log.ran.append(log.on[-1])
 
     class Graph:
         def replay(self):
             log.replays += 1
 
     @contextlib.contextmanager
-    def capture(graph, **kw):
-        yield
+    def capture(graph, stream=None, **kw):
+        log.captured.append(stream.role)
+        with on(stream):
+            yield
+    monkeypatch.setattr(streams, 'own', lambda dev, role: made.setdefault(role, Stream(role)))
+    monkeypatch.setattr(torch.cuda, 'stream', on)
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda device=None: Stream('caller'))
     monkeypatch.setattr(torch.cuda, 'CUDAGraph', Graph)
     monkeypatch.setattr(torch.cuda, 'graph', capture)
     monkeypatch.setattr(torch.cuda, 'graph_pool_handle', lambda: (0, 0))
     monkeypatch.setattr(torch.cuda, 'synchronize', lambda device=None: None)
     monkeypatch.setattr(graphs, '_prepare_capture', lambda dev: None)
-    monkeypatch.setattr(graphs.GraphedChain, '_body', lambda self, t: log.collector.append(gc.isenabled()))
+    monkeypatch.setattr(graphs.GraphedChain, '_body', body)
 
     def make(model, n=N):
         data = PlaceHolder(X=torch.zeros(B, n, KX), E=torch.zeros(B, n, n, KE), y=torch.zeros(B, 1), node_mask=torch.ones(B, n, dtype=torch.bool))
@@ -89,12 +115,12 @@ def test_no_collection_during_a_capture(chain):
     chain.make(model).run()
     assert chain.log.collector == [False] * T_EVAL and gc.isenabled()
     with pytest.raises(ZeroDivisionError):
-        with graphs._capture(torch.cuda.CUDAGraph()):
+        with graphs._capture(torch.cuda.CUDAGraph(), 'cuda:0'):
             1 / 0
     assert gc.isenabled()
     gc.disable()
     try:
-        with graphs._capture(torch.cuda.CUDAGraph()):
+        with graphs._capture(torch.cuda.CUDAGraph(), 'cuda:0'):
             pass
         assert not gc.isenabled()                                           # the caller's setting stays
     finally:
@@ -110,12 +136,37 @@ def test_a_chain_without_its_model_refuses(chain):
         c.run()
 
 
-def test_extra_features_are_not_captured(chain, monkeypatch):
-    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
-    monkeypatch.setattr(graphs, 'CHAIN_GRAPHS', '1')
-    assert graphs.chain_graphs_wanted(5, 40) and not graphs.chain_graphs_wanted(5, 40, extra_features=True)
+def test_a_new_chain_takes_no_pooled_stream(chain, monkeypatch):
+    """torch.cuda.Stream() walks through a pool of 32: a request per chain comes round to the capture stream.  Warm-up and capture each have a
+    stream of their own, which no other role shares."""
+    def pooled(*a, **k):
+        raise AssertionError('a stream out of the pool')
+    monkeypatch.setattr(torch.cuda, 'Stream', pooled)
     model = Model()
-    data = PlaceHolder(X=torch.zeros(B, N, KX), E=torch.zeros(B, N, N, KE), y=torch.zeros(B, 1), node_mask=torch.ones(B, N, dtype=torch.bool))
-    with pytest.raises(NotImplementedError, match='extra features'):
-        graphs.GraphedChain.get(model, data, (torch.ones(B, N, KX), torch.ones(B, N, N, KE)), None, (1.0, 1.0), None, None, True, 0)
-    assert len(model._chain_graphs) == 0
+    for n in range(2, 40):
+        c = chain.make(model, n)
+        c.warm = False
+        c.run()
+    assert set(chain.log.ran) == {'warm', 'capture'} and chain.log.ran.count('warm') == 38
+    assert set(chain.log.captured) == {'capture'}
+
+
+def test_no_pooled_streams_in_the_package():
+    root = os.path.dirname(graphs.__file__)
+    for name in os.listdir(root):
+        if name.endswith('.py'):
+            text = open(os.path.join(root, name)).read()
+            assert 'cuda.Stream(' not in re.sub(r'""".*?"""', '', text, flags=re.S), name
+    assert len(set(streams.ROLES)) == len(streams.ROLES)
+
+
+def test_streams_are_made_once_per_device(monkeypatch):
+    made = []
+    monkeypatch.setattr(streams, '_OWN', {})
+    monkeypatch.setattr(streams, '_create', lambda index: made.append(index) or object())
+    a = {r: streams.own('cuda:0', r) for r in streams.ROLES}
+    b = {r: streams.own(torch.device('cuda', 1), r) for r in streams.ROLES}
+    assert all(streams.own('cuda:0', r) is a[r] for r in streams.ROLES) and made == [0] * len(a) + [1] * len(b)
+    assert len({id(s) for s in (*a.values(), *b.values())}) == 2 * len(streams.ROLES)
+    with pytest.raises(KeyError):
+        streams.own('cuda:0', 'another')
