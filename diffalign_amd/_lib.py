@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get('DA_LIB') or os.path.join(_HERE, 'libdiffalign_hip.so'
 _lib: Optional[C.CDLL] = None
 
 c_f = C.c_void_p  # all device pointers travel as void*
-ABI_VERSION = 4      # DA_ABI_VERSION of include/diffalign_hip.h this binding was written against
+ABI_VERSION = 3      # DA_ABI_VERSION of include/diffalign_hip.h this binding was written against
 
 # Signatures of include/diffalign_hip.h, 'return:arguments' with p = pointer (void*), i = int, q = long long, f = float,
 # s = const char*; set on the library once, so that no call site can truncate a size or pass a float as a double

@@ -13,9 +13,9 @@ void da_set_error(const char* fmt, ...) {
 
 extern "C" {
 const char* da_last_error(void) { return g_err; }
-// 4: da_mx8_*, da_linear_wgrad_mx8, da_relu_dropout_bwd_mx8, da_attn_head_* added; 3: da_init added, the two-pass output stage (da_edge_out_g / da_edge_out_finish) removed; 2:
+// 3: da_init added, the two-pass output stage (da_edge_out_g / da_edge_out_finish) removed; 2:
 // da_y_film / da_y_update* take the y-chain weights k-major ((in, out)), da_edge_layer_stats resets its ticket word itself
-int da_abi_version(void) { return 4; }
+int da_abi_version(void) { return 3; }
 int da_stream_create(void** stream) {
   DA_CHECK_ARG(stream, "da_stream_create: null pointer");
   hipStream_t s = nullptr;

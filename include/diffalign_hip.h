@@ -17,10 +17,10 @@ extern "C" {
 #endif
 
 /* Version of this header's contracts; a binding built against another version must refuse the library (diffalign_amd/_lib.py does).
- * 4: 8-bit activation checkpoints (da_mx8_*, da_linear_wgrad_mx8, da_relu_dropout_bwd_mx8) and the per-head attention core (da_attn_head_*)
- * added.  3: da_init, the bf16-storage training kernels (da_attn_core_*_bf16, da_linear_wgrad_mixed) and the fused residual blocks (da_res_ln_*, da_relu_dropout*) added, da_edge_out_g / da_edge_out_finish / da_skip_grad removed.  2: da_y_film / da_y_update / da_y_update_film / da_y_pre expect the
+ * Since 3, additions only (no new number, a binding of 3 keeps working): 8-bit activation checkpoints (da_mx8_*, da_linear_wgrad_mx8,
+ * da_relu_dropout_bwd_mx8), the per-head attention core (da_attn_head_*), da_stream_create.  3: da_init, the bf16-storage training kernels (da_attn_core_*_bf16, da_linear_wgrad_mixed) and the fused residual blocks (da_res_ln_*, da_relu_dropout*) added, da_edge_out_g / da_edge_out_finish / da_skip_grad removed.  2: da_y_film / da_y_update / da_y_update_film / da_y_pre expect the
  * y-chain weights k-major, i.e. transposed to (in, out); da_edge_layer_stats puts its ticket word back to zero itself. */
-#define DA_ABI_VERSION 4
+#define DA_ABI_VERSION 3
 int da_abi_version(void);
 const char* da_last_error(void);
 /* Per-device set-up that must not run under stream capture (today: the device address of da_edge_in_sym_static's scratch).  Call once

@@ -170,3 +170,9 @@ def test_streams_are_made_once_per_device(monkeypatch):
     assert len({id(s) for s in (*a.values(), *b.values())}) == 2 * len(streams.ROLES)
     with pytest.raises(KeyError):
         streams.own('cuda:0', 'another')
+
+
+def test_stream_create_refuses_a_null_pointer_and_the_version_stays():
+    from diffalign_amd import _lib as L
+    assert L.lib().da_stream_create(None) != 0 and b'da_stream_create' in L.lib().da_last_error()
+    assert L.lib().da_abi_version() == 3                # entry points were only added: a binding of version 3 keeps loading
