@@ -26,6 +26,16 @@ def _once(backward):
     return lambda ctx, *grads: guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
 
+def _own_types(fn):
+    """fn outside the caller's autocast: the products below run in their operands' types, which the kernels beside them are called for."""
+    def run(ctx, *args):
+        if not torch.is_autocast_enabled('cuda'):
+            return fn(ctx, *args)
+        with torch.autocast('cuda', enabled=False):
+            return fn(ctx, *args)
+    return run
+
+
 def _c16(t):
     """contiguous fp32 at a 16-byte aligned address (kernels that read float4)."""
     t = _c(t)
@@ -125,6 +135,7 @@ class WideLinearMx8(Function):
     Linears of one input share it)."""
 
     @staticmethod
+    @_own_types
     def forward(ctx, x, weight, bias, codes, scales):
         w, b = (weight, bias) if x.dtype == torch.float32 else (weight.to(x.dtype), bias.to(x.dtype))
         ctx.save_for_backward(codes, scales, w)
@@ -132,6 +143,7 @@ class WideLinearMx8(Function):
 
     @staticmethod
     @_once
+    @_own_types
     def backward(ctx, dy):
         codes, scales, w = ctx.saved_tensors
         dy = dy.contiguous()
@@ -144,6 +156,7 @@ class FeedForwardMx8(Function):
     quantised so that what is not zero stays so: its codes are the ReLU's and the dropout's mask as well."""
 
     @staticmethod
+    @_own_types
     def forward(ctx, x, w1, b1, w2, b2, seed, salt, p):
         q = mx8.quantize(x)
         if x.dtype != torch.float32:
@@ -156,6 +169,7 @@ class FeedForwardMx8(Function):
 
     @staticmethod
     @_once
+    @_own_types
     def backward(ctx, dy):
         codes, scales, hc, hs, w1, w2 = ctx.saved_tensors
         dy = dy.contiguous()
@@ -180,6 +194,8 @@ def feed_forward(lin1: torch.nn.Linear, lin2: torch.nn.Linear, x: torch.Tensor, 
 
 def _relu_dropout_(h, seed, salt, p):
     p = float(p)
+    if h.dtype not in (torch.float32, torch.bfloat16):        # (fp16 under a caller's autocast: the kernel would take it for fp32)
+        raise L.DiffAlignHipError(f'relu_dropout: fp32 or bf16 expected, got {h.dtype}')
     L.check(L.lib().da_relu_dropout(L.ptr(h), int(h.dtype == torch.bfloat16), h.numel(), L.ptr(seed if p > 0 else None), salt, p, L.stream()),
             'da_relu_dropout')
     return h

@@ -35,6 +35,14 @@ def test_refusals():
         L._held.clear()
 
 
+def test_relu_dropout_refuses_other_types():
+    """fp16 (the result of a Linear under a caller's fp16 autocast) would be read and written as twice as many bytes."""
+    from diffalign_amd import autograd_ops as A, _lib as L
+    for dtype in (torch.float16, torch.float64):
+        with pytest.raises(L.DiffAlignHipError, match='fp32 or bf16'):
+            A._relu_dropout_(torch.zeros(4, 8, dtype=dtype), None, 0, 0.0)
+
+
 def test_c_entries_refuse_before_any_launch():
     """Argument checks of the C entry points: they return before anything is launched, so they run without a GPU."""
     from diffalign_amd import _lib as L
