@@ -115,8 +115,9 @@ __global__ void __launch_bounds__(256) k_relu_drop_bwd_mx8_any(const int8_t* __r
 // keeps the whole (OUT,IN) result in accumulators, and the slices' partial results are folded in slice order (no atomics).
 // v_mfma_f32_32x32x16_bf16 sums over 16 rows at a time and wants 8 rows of one feature per lane, while memory is contiguous along the
 // features: tiles of KR rows go through LDS row-major and come back through the transposing read (ds_read_b64_tr_b16: 4 rows of 16
-// features per 16 lanes).  x^ = q 2^e is exact in bf16.  dY: bf16 as it is; fp32 as the sum of three bf16 parts (8 + 8 + 8 bits: the
-// whole significand), one product each, so nothing of it is rounded away.  Products are exact, sums fp32.
+// features per 16 lanes).  x^ = q 2^e is exact in bf16.  dY: bf16 as it is; fp32 as the sum of three bf16 parts (8 + 8 + 8 bits, each cut
+// toward zero: the whole significand, down to the 2^-126 below which a part is a subnormal), one product each, so nothing of it is rounded
+// away.  Products are exact, sums fp32.
 // A tile's next rows are loaded into registers while the matrix instructions of the present one run (a second LDS buffer in place of the second
 // barrier changes nothing).  313,600 rows: 64 -> 256 bf16 40 us (181 MB, 4.5 TB/s), 256 -> 64 fp32 50 us (163 MB, 3.3 TB/s: three products
 // and 256 conversions a row beside the stream), and 8 us for the fold of 512 partial results.
@@ -138,6 +139,10 @@ struct WgradCfg {
   static constexpr int NXT = KR * IN / 8;
   static constexpr int CY = (NYT + 255) / 256, CX = (NXT + 255) / 256;
 };
+// the upper halves of two floats: bf16 cut toward zero, so that no finite value becomes infinite (rounded to nearest, 3.3953e38 and more does)
+__device__ __forceinline__ unsigned hi_bf16(float a, float b) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+}
 typedef __attribute__((ext_vector_type(4))) short i16x4;
 __device__ __forceinline__ bf16x8 tr_frag(const char* base, int pitch, int row, int feat, int lane) {
   // rows row + 8 h .. + 7 (two reads of 4), features feat .. feat + 31: lane i of 16 addresses row i / 4, features 4 (i % 4) ..
@@ -208,13 +213,15 @@ __global__ void __launch_bounds__(256) k_mx8_wgrad(const uint8_t* __restrict__ c
       char* d = s_y + row * C::PY + f * 2;
 #pragma unroll
       for (int pl = 0; pl < C::PLANES; ++pl) {
-        uint4 o = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+        uint4 o;
+        if constexpr (C::PLANES == 1) o = uint4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+        else o = uint4{hi_bf16(v[0], v[1]), hi_bf16(v[2], v[3]), hi_bf16(v[4], v[5]), hi_bf16(v[6], v[7])};
         *reinterpret_cast<uint4*>(d + pl * C::Y_BYTES) = o;
-        if (pl + 1 < C::PLANES) {                                      // what this part leaves, exactly
+        if (pl + 1 < C::PLANES) {                                      // what this part leaves, exactly; nothing of an infinity, NaN of a NaN
           float p8[8];
           unpack8(o, p8);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) { const float d = v[k] - p8[k]; v[k] = d == d ? d : 0.f; }      // (inf, NaN: all in the first part)
+          for (int k = 0; k < 8; ++k) v[k] = v[k] == p8[k] ? 0.f : v[k] - p8[k];
         }
       }
     }

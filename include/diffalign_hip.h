@@ -229,8 +229,9 @@ int da_mx8_dequant(const void* codes, const uint8_t* scales, void* out, int out_
 /* da_relu_dropout_bwd from the codes (numel int8, quantised with keep_nonzero) of the stored result. */
 int da_relu_dropout_bwd_mx8(const void* codes, const void* dy, void* dx, int is_bf16, long long numel, float p, void* stream);
 /* da_linear_wgrad with X (R, in) held in 8 bits: dW (out,in) = dY^T X, db (out) = column sums of dY (NULL: skipped), fp32.  dY fp32 or bf16
- * (dy_bf16), every product exact, sums fp32, slices folded in order (deterministic).  in, out in {32, 64, 128, 256} with in * out <= 16384
- * (others: DA_ERR_UNSUPPORTED, workspace -1); dY, dW, db, workspace 16-byte, codes 8-byte aligned; R >= 1. */
+ * (dy_bf16), every product exact (of an fp32 dY what is below 2^-125 may be lost), sums fp32, slices folded in order (deterministic).
+ * in, out in {32, 64, 128, 256} with in * out <= 16384 (others: DA_ERR_UNSUPPORTED, workspace -1); dY, dW, db, workspace 16-byte, codes
+ * 8-byte aligned; R >= 1. */
 long long da_linear_wgrad_mx8_workspace(long long R, int in_features, int out_features);
 int da_linear_wgrad_mx8(const void* codes, const uint8_t* scales, const void* dY, int dy_bf16, float* dW, float* db, void* workspace,
                         long long workspace_bytes, long long R, int in_features, int out_features, void* stream);
