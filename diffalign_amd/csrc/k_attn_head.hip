@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
     for (int t = 0; t < RW; ++t) {
       float e1[C], G[C], o1[C], o2[C], dp = 0.f;
       if constexpr (MX8) {
-        const float step = mx8_step(op[t].sc < MX8_B_MIN ? MX8_B_MIN : op[t].sc);          // (a masked pair reads 0)
+        const float step = mx8_step(op[t].sc);                            // (a masked pair reads 0, and codes of 0)
 #pragma unroll
         for (int k = 0; k < C; k += 4) {
           e1[k] = mx8_elem<0>(op[t].e1[k / 4]) * step; e1[k + 1] = mx8_elem<1>(op[t].e1[k / 4]) * step;

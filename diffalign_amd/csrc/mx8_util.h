@@ -1,7 +1,8 @@
 // MXINT8 (OCP microscaling): 32 consecutive channels of a row share a power-of-two scale X = 2^(b - 127), one byte b; an element is an
 // int8 q and stands for q / 64 * X.  b is the smallest exponent at which the group's largest magnitude rounds to 127 or less, so
 // every value is within half a step, X / 128, of its element (an amax over 127.5 / 64 * 2^127 has no such b and saturates at 127).
-// b is held in [MX8_B_MIN, 254]: X >= 2^-100 keeps every element a normal bf16 / fp32, which the matrix instructions do not flush.
+// b as written is in [MX8_B_MIN, 254]: X >= 2^-100 keeps every element a normal bf16 / fp32 (smaller values round to zero at that step); any
+// byte is read.
 // A group with an infinity or NaN gets b = 255 and stands for NaN throughout.  An element has 7 significant bits: exact in bf16.
 #pragma once
 #include "common.h"
@@ -17,8 +18,11 @@ __device__ __forceinline__ unsigned mx8_scale(unsigned amax_bits) {
 }
 // 64 / X: what a value is multiplied by; 0 for the NaN group (its codes are 0)
 __device__ __forceinline__ float mx8_inv(unsigned b) { return __builtin_bit_cast(float, b == 255u ? 0u : (260u - b) << 23); }
-// X / 64: what a code stands for
-__device__ __forceinline__ float mx8_step(unsigned b) { return __builtin_bit_cast(float, b == 255u ? 0x7fc00000u : (b - 6u) << 23); }
+// X / 64 = 2^(b - 133): what a code stands for.  A caller's own scale bytes may lie below MX8_B_MIN: up to 6 the step is a subnormal, of which
+// fp32 holds every multiple by a code exactly
+__device__ __forceinline__ float mx8_step(unsigned b) {
+  return __builtin_bit_cast(float, b == 255u ? 0x7fc00000u : b < 7u ? 0x10000u << b : (b - 6u) << 23);
+}
 // round to nearest even of x * inv in the low byte of a word: 1.5 * 2^23 has a unit of 1 and x * inv is exact (a power of two) unless it is
 // far below one half, so the fused sum rounds once.  The clamp acts only where the scale is saturated (or x is not finite: inv = 0, and
 // that group's codes are 0).

@@ -218,8 +218,9 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
                      long long workspace_bytes, int B, int n, int dx, int n_head, void* stream);
 /* ---- 8-bit activation checkpoints of the training step (the reference keeps full-width activations for loss.backward(),
  * training/helpers.py:139-142).  MXINT8: 32 consecutive channels of a row share the scale 2^(b-127) (one byte b), an element is an int8 q and
- * stands for q / 64 * 2^(b-127); b is the smallest in [27, 254] at which the group's largest magnitude rounds to 127 or less, 255 (the
- * group stands for NaN, whatever its codes) where the group holds an infinity or NaN.  codes (rows, D), scales (rows, ceil(D / 32)). ---- */
+ * stands for q / 64 * 2^(b-127); written, b is the smallest in [27, 254] at which the group's largest magnitude rounds to 127 or less, 255
+ * (the group stands for NaN, whatever its codes) where the group holds an infinity or NaN; read, it may be any byte.  codes (rows, D),
+ * scales (rows, ceil(D / 32)). ---- */
 
 /* Quantise x (rows, D) fp32 or bf16 (x_bf16).  keep_nonzero: an element other than zero gets a code other than zero.  Any D >= 1; D % 32
  * == 0 with x 16-byte and codes 8-byte aligned takes the wide path. */
@@ -229,7 +230,7 @@ int da_mx8_dequant(const void* codes, const uint8_t* scales, void* out, int out_
 /* da_relu_dropout_bwd from the codes (numel int8, quantised with keep_nonzero) of the stored result. */
 int da_relu_dropout_bwd_mx8(const void* codes, const void* dy, void* dx, int is_bf16, long long numel, float p, void* stream);
 /* da_linear_wgrad with X (R, in) held in 8 bits: dW (out,in) = dY^T X, db (out) = column sums of dY (NULL: skipped), fp32.  dY fp32 or bf16
- * (dy_bf16), every product exact (of an fp32 dY what is below 2^-125 may be lost), sums fp32, slices folded in order (deterministic).
+ * (dy_bf16), every product exact (of an fp32 dY bits below 2^-133 are cut), sums fp32, slices folded in order (deterministic).
  * in, out in {32, 64, 128, 256} with in * out <= 16384 (others: DA_ERR_UNSUPPORTED, workspace -1); dY, dW, db, workspace 16-byte, codes
  * 8-byte aligned; R >= 1. */
 long long da_linear_wgrad_mx8_workspace(long long R, int in_features, int out_features);

@@ -49,8 +49,8 @@ def test_linear_wgrad_of_infinite_and_nan_gradients():
 
 
 def test_linear_wgrad_of_tiny_gradients():
-    """fp32 dY down to the smallest normal beside a large x.  A part of dY below 2^-126 is a subnormal bf16, and what a bf16 cannot hold at all is
-    lost: less than 2^-125 |x| a product."""
+    """fp32 dY down to the smallest normal beside a large x.  A part of dY below 2^-126 is a subnormal bf16, which the matrix instruction takes as
+    it is, and what no bf16 holds is lost: less than 2^-133 |x| a product."""
     from diffalign_amd import mx8
     g = torch.Generator().manual_seed(8)
     R = 200
@@ -58,4 +58,40 @@ def test_linear_wgrad_of_tiny_gradients():
     dy = torch.randn(R, 64, generator=g) * torch.exp2(-126 + 30 * torch.rand(R, 1, generator=g))
     dW, db = mx8.linear_wgrad(mx8.Mx8(codes.to(D_), scales.to(D_)), dy.to(D_))
     d = dy.double()
-    assert bool(((dW.cpu().double() - d.t() @ x).abs() <= SMALL * (d.abs().t() @ x.abs()) + 2.0 ** -125 * x.abs().sum(0)).all())
+    assert bool(((dW.cpu().double() - d.t() @ x).abs() <= SMALL * (d.abs().t() @ x.abs()) + 2.0 ** -133 * x.abs().sum(0)).all())
+
+
+def small_scales(rows, D, seed, most=31):
+    """Codes with every scale byte a caller's own 8-bit data may have: 0 to 26 are not written by quantize."""
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-127, 128, (rows, D), generator=g).to(torch.int8)
+    G = -(-D // 32)
+    scales = (torch.arange(rows * G) % most).reshape(rows, G).to(torch.uint8)
+    vals = codes.double() * torch.exp2(scales.double() - 133).repeat_interleave(32, 1)[:, :D]
+    return codes, scales, vals
+
+
+@pytest.mark.parametrize('rows,D', [(37, 64), (19, 33), (40, 256)])
+def test_scale_bytes_from_zero(rows, D):
+    """The scale byte b stands for 2^(b - 127) from 0 on, 255 for NaN; the values, subnormal or not, are exact in fp32 and bf16."""
+    from diffalign_amd import mx8
+    codes, scales, vals = small_scales(rows, D, 1)
+    q = mx8.Mx8(codes.to(D_), scales.to(D_))
+    for out in (torch.float32, torch.bfloat16):
+        assert torch.equal(mx8.dequantize(q, out).cpu().double(), vals)
+    scales[3] = 255
+    got = mx8.dequantize(mx8.Mx8(codes.to(D_), scales.to(D_))).cpu()
+    assert bool(got[3].isnan().all()) and torch.equal(torch.cat((got[:3], got[4:])).double(), torch.cat((vals[:3], vals[4:])))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('most', [5, 31])
+def test_linear_wgrad_of_scale_bytes_from_zero(most, dtype):
+    """Small x (up to byte 4: subnormal throughout) beside a dY that makes up for it."""
+    from diffalign_amd import mx8
+    codes, scales, x = small_scales(200, 64, 2, most)
+    dy = (act(200, 128, torch.float32, 7) * 2.0 ** 90).to(dtype)
+    dW, db = mx8.linear_wgrad(mx8.Mx8(codes.to(D_), scales.to(D_)), dy.to(D_))
+    d = dy.double()
+    assert bool(((dW.cpu().double() - d.t() @ x).abs() <= SMALL * (d.abs().t() @ x.abs())).all())
+    assert bool(((db.cpu().double() - d.sum(0)).abs() <= SMALL * d.abs().sum(0)).all())
