@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(64 * HEAD_NW) k_attn_head_bwd(HeadArgs a) {
         const float x = fma_(G[k], e1[k], G[k]);
         dq[t][k] = fma_(x, kk[k], dq[t][k]);
         dk[k] = fma_(x, q[t][k], dk[k]);
-        dv[k] = fma_(p, g[t][k], dv[k]);
+        dv[k] = fma_(p, on ? g[t][k] : 0.f, dv[k]);                     // (an unseen key: the row's dwV is not looked at)
       }
       bst<TY, C>(r1o, oE + t * row_e, o1); bst<TY, C>(r2o, oE + t * row_e, o2);
       __builtin_amdgcn_sched_barrier(0);                                // one row's temporaries at a time: mixed, the rows spill

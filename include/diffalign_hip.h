@@ -210,7 +210,7 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
                      int n, int dx, int n_head, void* stream);
 /* From dY (B,n,n,dx) fp32 or bf16 (dy_bf16) and dwV (B,n,dx) to dQ, dK, dV fp32, dE1, dE2 of dY's type (0 where m_ij = 0).  E1 of dY's type, or
  * NULL with its codes and scales.  wV, S, stat as the forward left them; workspace (da_attn_head_bwd_workspace bytes, -1: not built) holds
- * partial dQ, dK, dV, folded in order (deterministic). */
+ * partial dQ, dK, dV, folded in order (deterministic).  dwV of a row has no effect on dV of a key that the row does not see. */
 long long da_attn_head_bwd_workspace(int B, int n, int dx, int n_head, int dy_bf16);
 int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void* E1, const void* E1_codes, const uint8_t* E1_scales,
                      const uint8_t* node_mask, float qscale, float cap, const float* wV, const float* S, const float* stat, const void* dY,
