@@ -179,6 +179,6 @@ def stream() -> C.c_void_p:
 
 
 def as_u8(mask: torch.Tensor) -> torch.Tensor:
-    """bool -> uint8 view (no copy)."""
+    """bool -> uint8 view (no copy; a copy where torch.jit.trace records, which takes no view of another type)."""
     m = mask.contiguous()
-    return m.view(torch.uint8) if m.dtype == torch.bool else m.to(torch.uint8)
+    return m.view(torch.uint8) if m.dtype == torch.bool and torch._C._get_tracing_state() is None else m.to(torch.uint8)

@@ -8,7 +8,7 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -360,7 +360,8 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
     E1 and E2 are not looked at where a node of the pair is masked.  The softmax runs over all keys, as in the reference, or with `groups`
     (B,n) integers below 2^31 over the keys of the query's own group (a node with a negative group is in none: its wV is 0, and so is the
     wV of every row without a key; V of keys outside the group, or with a score of -inf, has no effect).  checkpoint='mx8': the backward gets E1 in 8 bits (mx8.py; needs dx % 32 == 0), which dQ and dK see.
-    fp32 arithmetic throughout; sums do not depend on timing."""
+    fp32 arithmetic throughout; sums do not depend on timing.  Differentiable once and backwards; forward-mode tangents are refused.  A call that
+    torch.jit.trace records is bound to the shapes it was traced with."""
     shape = Q.shape
     if len(shape) != 3 or K.shape != shape or V.shape != shape:
         raise L.DiffAlignHipError(f'head_attention: Q, K, V (B,n,dx) expected, got {tuple(shape)}, {tuple(K.shape)}, {tuple(V.shape)}')
@@ -390,7 +391,9 @@ def head_attention(Q, K, V, E1, E2, node_mask, n_head, qscale=None, cap=0.0, gro
     args = (mx8.aligned(Q.float()), mx8.aligned(K.float()), mx8.aligned(V.float()), mx8.aligned(E1), mx8.aligned(E2), L.as_u8(node_mask),
             None if groups is None else groups.to(torch.int32).contiguous(), n_head, qscale_of(dx, n_head) if qscale is None else float(qscale), cap,
             checkpoint == 'mx8', save)
-    return HeadAttnCore.apply(*args) if save else HeadAttnCore.forward(None, *args)
+    # past autograd (8 us of host time) only where nothing looks on: forward-mode differentiation has its refusal from apply, a trace its node
+    watched = save or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+    return HeadAttnCore.apply(*args) if watched else HeadAttnCore.forward(None, *args)
 
 
 class AddLayerNorm(Function):

@@ -7,7 +7,9 @@ largest magnitude); restored values are exact in bfloat16.  Scales go down to 2^
 group that holds an infinity or NaN is restored as NaN.  D channels take D + ceil(D / 32) bytes.
 
 The reference keeps every activation at full width for `loss.backward()` (training/helpers.py:139-142); the callers here are the training
-forward's per-pair Linears and the per-head attention core (train_forward.py, `train_checkpoint = 'mx8'`)."""
+forward's per-pair Linears and the per-head attention core (train_forward.py, `train_checkpoint = 'mx8'`).  The functions here are what
+those callers' forward and backward are made of and stand outside autograd: results carry no gradient and no tangent, and a
+torch.jit.trace does not see them."""
 from __future__ import annotations
 
 from typing import NamedTuple, Tuple
