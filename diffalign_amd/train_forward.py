@@ -120,21 +120,24 @@ def _node_edge_block_improved(a, X, E, y, nm_u8, xm, em, Eb=None, lanes=None, fu
 
 
 def _head_attention_torch(a, Q, K, V, E1, E2, em, groups):
-    """head_attention for head widths it is not built for, in torch operations."""
+    """head_attention for head widths it is not built for, in torch operations: like there, nothing is computed from what a mask, a group or a
+    score of -inf leaves out (a product with 0 would keep its NaN and infinities)."""
     B, n, dx = Q.shape
     H, df = a.n_head, a.df
+    zero = torch.zeros((), device=Q.device)
+    pm = em != 0
     Y = Q[:, :, None, :] * K[:, None, :, :] * qscale_of(dx, H)                                 # (B,i,j,dx)
-    Y = Y * (E1.float() * em + 1) + E2.float() * em                                           # :115-122
+    Y = Y * (torch.where(pm, E1.float(), zero) + 1) + torch.where(pm, E2.float(), zero)       # :115-122
     S = Y.reshape(B, n, n, H, df).sum(-1)
     if a.score_cap > 0:
         S = a.score_cap * torch.tanh(S / a.score_cap)
+    on = S != float('-inf')
     if groups is not None:
-        on = ((groups[:, :, None] == groups[:, None, :]) & (groups >= 0)[:, :, None])[..., None]
-        some = on.any(2, keepdim=True)                                                        # a row without a key: 0
-        attn = torch.softmax(torch.where(on | ~some, S, float('-inf')), dim=2) * some
-    else:
-        attn = torch.softmax(S, dim=2)                                                        # :128-130 (over keys, no mask)
-    wV = torch.einsum('bijh,bjhf->bihf', attn, V.reshape(B, n, H, df)).reshape(B, n, dx)      # :132-141
+        on = on & ((groups[:, :, None] == groups[:, None, :]) & (groups >= 0)[:, :, None])[..., None]
+    some = on.any(2, keepdim=True)                                                            # a row without a key: 0
+    S = torch.where(on, S, torch.where(some, float('-inf'), 0.0).to(S.dtype))
+    attn = torch.where(on, torch.softmax(S, dim=2), zero)                                     # :128-130 (over keys, no mask)
+    wV = (attn[..., None] * torch.where(on[..., None], V.reshape(B, 1, n, H, df), zero)).sum(2).reshape(B, n, dx)      # :132-141
     return Y.to(E1.dtype), wV
 
 
