@@ -494,13 +494,18 @@ static void head_chunks(int B, int n, int C, int lp_log, bool bf16, int* nib, in
   }
 }
 
+// rows per workgroup: 2 share K_j and V_j (3 and 4 take registers that are waves: 194 against 199 and 213 us, 1 row 226 us, bf16 B = 8, n = 300)
+// where that still gives 2 workgroups per CU, else 1
+#define HEAD_WIDE 2
+static int fwd_rows(int B, int n) { return (long long)B * ((n + HEAD_WIDE - 1) / HEAD_WIDE) >= 512 ? HEAD_WIDE : 1; }
+// a launch has fewer than 2^32 threads
+static bool fits_grid(long long groups, int threads) { return groups * threads < (1LL << 32); }
+
 template <class TE, int C, int HLOG>
 static void fwd_launch(const HeadArgs& a, bool save, bool mx8, hipStream_t s) {
-  // rows per workgroup: 2 share K_j and V_j (3 and 4 take registers that are waves: 194 against 199 and 213 us, 1 row 226 us, bf16 B = 8, n = 300)
-  // where that still gives 2 workgroups per CU, else 1
-  constexpr int WIDE = 2;
-  const bool wide = (long long)a.B * ((a.n + WIDE - 1) / WIDE) >= 512;
-  const int RW = wide ? WIDE : 1;
+  constexpr int WIDE = HEAD_WIDE;
+  const int RW = fwd_rows(a.B, a.n);
+  const bool wide = RW == WIDE;
   const long long grid = (long long)a.B * ((a.n + RW - 1) / RW);
   const size_t lds = sizeof(float) * 4 * RW * (a.dx + 2 * a.H);
 #define F(R, S, M) k_attn_head_fwd<TE, C, HLOG, R, S, M><<<(unsigned)grid, 256, lds, s>>>(a)
@@ -552,6 +557,8 @@ int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void*
   if (int rc = head_sizes("da_attn_head_fwd", B, n, dx, n_head, e_bf16 != 0, &C, &hlog, &a.lp_log)) return rc;
   if (B == 0 || n == 0) return DA_OK;
   DA_CHECK_ARG(Q && K && V && E1 && E2 && node_mask && Y && wV, "da_attn_head_fwd: null pointer");
+  const int RW = fwd_rows(B, n);
+  DA_CHECK_ARG(fits_grid((long long)B * ((n + RW - 1) / RW), 256), "da_attn_head_fwd: B = %d, n = %d too large for one launch", B, n);
   DA_CHECK_ARG((S == nullptr) == (stat == nullptr) && (E1_codes == nullptr) == (E1_scales == nullptr) && (!E1_codes || S),
                "da_attn_head_fwd: S and stat go together, E1's codes and scales with both");
   DA_CHECK_ARG(!E1_codes || dx % MX8_GROUP == 0, "da_attn_head_fwd: 8-bit E1 needs dx %% 32 == 0, dx = %d", dx);
@@ -594,6 +601,7 @@ int da_attn_head_bwd(const float* Q, const float* K, const float* V, const void*
   a.Q = Q; a.K = K; a.V = V; a.E1 = E1_codes ? E1_codes : E1; a.E1s = E1_scales; a.nm = node_mask; a.qscale = qscale; a.cap = cap; a.n = n; a.dx = dx;
   a.H = n_head; a.wV = (float*)wV; a.S = (float*)S; a.stat = (float*)stat; a.dY = dY; a.dwV = dwV; a.dE1 = dE1; a.dE2 = dE2; a.B = B;
   head_chunks(B, n, C, a.lp_log, dy_bf16 != 0, &a.nib, &a.njc, &a.jchunk);
+  DA_CHECK_ARG(fits_grid((long long)B * a.nib * a.njc, 64 * HEAD_NW), "da_attn_head_bwd: B = %d, n = %d too large for one launch", B, n);
   const size_t one = (size_t)B * n * dx;
   float* ws = (float*)workspace;
   a.dKp = dK; a.dVp = dV; a.dQp = dQ;

@@ -204,7 +204,7 @@ int da_relu_dropout_bwd(const void* h, const void* dy, void* dx, int is_bf16, lo
  * Q, K, V, wV (B,n,dx) fp32; E1, E2, Y (B,n,n,dx) fp32 or bf16 (e_bf16).  For a backward: S (B,n,n,n_head) fp32 and stat (B,n,n_head,2) are
  * written when given (both or neither), and E1_codes / E1_scales get E1 in 8 bits (da_mx8_quant's format; dx % 32 == 0).
  * Built: 4, 8, 16, .. 128 channels per head, dx <= 512 (256 with 4 channels per head); others: DA_ERR_UNSUPPORTED.  Tensors 16-byte aligned (stat 8,
- * S 4, the bytes any). */
+ * S 4, the bytes any).  One launch: B < 2^24 graphs of one node forward, 2^23 backward (fewer threads than 2^32), else DA_ERR_ARG. */
 int da_attn_head_fwd(const float* Q, const float* K, const float* V, const void* E1, const void* E2, int e_bf16, const uint8_t* node_mask,
                      const int* groups, float qscale, float cap, void* Y, float* wV, float* S, float* stat, void* E1_codes, uint8_t* E1_scales, int B,
                      int n, int dx, int n_head, void* stream);

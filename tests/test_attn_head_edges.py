@@ -67,3 +67,13 @@ def test_torch_form_shuts_out_scores_of_minus_infinity(shut, groups):
     P = torch.softmax((torch.einsum('ihc,jhc->ijhc', q, k) / 6 ** 0.5 * (1 + e1) + e2).sum(-1), 1)
     want = torch.einsum('ijh,jhc->ihc', P, v).reshape(6, 12)
     assert float((got[1][0, rows].double() - want).abs().max()) <= 1e-5 * float(want.abs().max())
+
+
+def test_c_entries_refuse_more_than_a_launch_holds():
+    """2^32 threads and more, which no launch takes: refused before anything is launched, with the sizes in the message."""
+    from diffalign_amd import _lib as L
+    lib, p = L.lib(), 16
+    fwd = lambda B, n: lib.da_attn_head_fwd(p, p, p, p, p, 0, p, 0, 1.0, 0.0, p, p, 0, 0, 0, 0, B, n, 64, 4, 0)
+    bwd = lambda B, n: lib.da_attn_head_bwd(p, p, p, p, 0, 0, p, 1.0, 0.0, p, p, p, p, 0, p, p, p, p, p, p, p, 1 << 60, B, n, 64, 4, 0)
+    for call, B, n in ((fwd, 1 << 24, 1), (fwd, 1 << 23, 3), (bwd, 1 << 23, 1), (bwd, 1 << 21, 100)):
+        assert call(B, n) == -1 and b'launch' in lib.da_last_error() and str(B).encode() in lib.da_last_error()
