@@ -317,6 +317,9 @@ def forward_train(m, X, E, y, node_mask, atom_map_numbers=None, pos_encodings=No
     Eb = None
     for k, layer in enumerate(m.tf_layers):
         fuse = (seed, 16 * k) if fused and _fusable(layer, Xh, Eh, yh, checkpoint) else None
+        if checkpoint == 'mx8' and fuse is None:
+            raise ValueError(f"train checkpoint 'mx8' goes with the fused residual blocks: rows of {Xh.shape[-1]}, {Eh.shape[-1]} and {yh.shape[-1]} channels "
+                             f'(built: {sorted(FUSED_WIDTHS)}), hidden sizes divisible by 4')
         Xh, Eh, yh, Eb = _layer(layer, Xh, Eh, yh, nm_u8, xm, em, m.training, bf16, lanes, Eb, fuse, checkpoint, groups)
     lanes.to_pair(Xh, yh)
     kx, ke, ky = m.out_dim_X, m.out_dim_E, m.out_dim_y
