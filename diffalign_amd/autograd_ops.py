@@ -48,7 +48,11 @@ _WS = {}
 def _workspace(device, nbytes: int) -> torch.Tensor:
     """Grow-only scratch per (device, stream) for the two-stage kernels (partial results): calls on one stream are ordered, so they
     share it; the node and pair sides of the training step run on two streams (train_forward.py) and must not.  A buffer that is
-    outgrown is handed back through the allocator, which defers its reuse behind the stream's pending work."""
+    outgrown is handed back through the allocator, which defers its reuse behind the stream's pending work.
+    A graph being recorded gets memory of its own: it keeps the address for its replays, which know nothing of a buffer that was outgrown since,
+    and run beside eager work and other graphs."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
     key = (device, torch.cuda.current_stream(device).cuda_stream)
     w = _WS.get(key)
     if w is None or w.numel() < nbytes:
