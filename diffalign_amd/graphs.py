@@ -62,6 +62,21 @@ def chain_graphs_wanted(B: int, n: int) -> bool:
     return CHAIN_GRAPHS == '1' or B * n * n <= CHAIN_GRAPH_MAX_PAIRS
 
 
+def _in_a_live_graph(params) -> list:
+    """Those of `params` (leaves) that an autograd graph still refers to: such a graph keeps the leaf's accumulation node, and a backward
+    pass that is recorded takes that node with the stream it was made on, outside the recording, which ends the process.  (A node without
+    a graph goes as soon as it is let go, so a mark on it does not last.)"""
+    def node(p):
+        with torch.enable_grad():
+            return p.expand_as(p).grad_fn.next_functions[0][0]
+    held = []
+    for p in params:
+        node(p).metadata['diffalign_amd'] = True
+        if node(p).metadata.pop('diffalign_amd', False):
+            held.append(p)
+    return held
+
+
 class GraphedTrainStep:
     """One whole training step -- apply_noise, apply_mask, extra features, the differentiable fp32 forward, the objective, backward(),
     the gradient gather, (the data-parallel all-reduce) and the fused AdamW -- captured once as a HIP graph and replayed per batch.
@@ -74,11 +89,16 @@ class GraphedTrainStep:
     Building the object does not train: the `warmup` eager steps (they settle allocator pools, workspaces and lazily built tables)
     and the capture pass run on the example batch, and the weights, both moments, the device step counter and the host's `steps` are
     put back to what they were afterwards (torch's generator state is consumed).  After N calls opt.steps == int(opt.step_dev)
-    == the count before construction + N."""
+    == the count before construction + N.  No autograd graph of the parameters may be alive at construction (a loss or logits of an
+    eager training_step, detached ones aside): it raises."""
 
     def __init__(self, model, optimizer, example: PlaceHolder, warmup: int = 3, group=None):
         assert optimizer.step_dev is not None, 'GraphedTrainStep needs optim.FlatAdamW(..., device_step=True)'
         assert model.model.training, 'call model.train() first'
+        if _in_a_live_graph(optimizer.params):
+            gc.collect()                                     # (graphs that only a reference cycle holds)
+            if _in_a_live_graph(optimizer.params):
+                raise RuntimeError('GraphedTrainStep: an autograd graph of these parameters is alive (a loss or logits of an earlier eager pass); let it go first')
         self.model, self.opt, self.group = model, optimizer, group
         _prepare_capture(example.X.device)
         self.data = example.get_new_object()                 # static copies (get_new_object clones every field)
