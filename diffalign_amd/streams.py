@@ -3,8 +3,9 @@
 torch.cuda.Stream() hands out the 32 streams of a per-device pool in turn: the 33rd call returns the first one's stream again.  A stream asked
 for per chain or per call walks through the pool, and after 32 the 'new' stream is torch's graph capture stream, or one of the side
 streams whose work it is meant to be ordered against -- eager work then runs on the stream a graph is recorded on next, and a captured fork
-joins the stream it forked from.  (Replaying graphs recorded over several streams ended the process, a segmentation fault in the runtime's graph
-launch, at exactly the call where the pool came round to the capture stream.)  Streams made here are nobody else's."""
+joins the stream it forked from.  (Graph launches ended the process, a segmentation fault in the runtime, three times: each after eager forked
+work on the stream that earlier graphs had been recorded on and the next one was.  Most likely that is the cause; what the runtime does there
+is not known.)  Streams made here are nobody else's."""
 from __future__ import annotations
 
 import ctypes as C

@@ -265,8 +265,6 @@ def test_config2_shape_100_steps_100_samples_one_condition():
     assert len({tuple(r.tolist()) for r in a.X.cpu()[:, :s]}) > 1         # chains are not copies of each other
 
 
-@pytest.mark.skip(reason='ended the process twice (host segmentation fault in the graph launch) behind 303 other tests, where a pooled stream '
-                         'came round to the capture stream; the streams are the framework\'s own since (streams.py), the test has not been run again')
 def test_graphed_chain_equals_eager_chain():
     """graphs.GraphedChain: every reverse step of a small batch replayed as a HIP graph (three-stream arrangement captured, extra
     features with the eigensolver's fixed-block cache inside, counter noise, inpainting) gives the eager loop's samples bit for bit;
