@@ -95,3 +95,24 @@ def test_linear_wgrad_of_scale_bytes_from_zero(most, dtype):
     d = dy.double()
     assert bool(((dW.cpu().double() - d.t() @ x).abs() <= SMALL * (d.abs().t() @ x.abs())).all())
     assert bool(((db.cpu().double() - d.sum(0)).abs() <= SMALL * d.abs().sum(0)).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['fp32', 'bf16'])
+@pytest.mark.parametrize('shape', [(64, 256), (256, 64), (32, 32), (128, 64)], ids=lambda s: f'{s[0]}-{s[1]}')
+@pytest.mark.parametrize('R', [60_001, 140_001])
+def test_linear_wgrad_rows_of_a_training_batch(R, shape, dtype):
+    """Slices of several tiles with data in every row, on both sides of the change of the number of slices, the last slice ragged."""
+    from diffalign_amd import mx8
+    i, o = shape
+    g = torch.Generator(device=D_).manual_seed(R + i)
+    q = mx8.quantize(torch.randn(R, i, device=D_, generator=g) * torch.exp(torch.randn(R, 1, device=D_, generator=g)))
+    dy = torch.randn(R, o, device=D_, generator=g).to(dtype)
+    dW, db = mx8.linear_wgrad(q, dy)
+    x, d = mx8.dequantize(q).double(), dy.double()
+    slice_rows = 256 if R == 60_001 else 320
+    parts = -(-R // slice_rows) * (4 if i * o == 1024 else 1)                                 # 32 -> 32: four waves over a slice's rows
+    tol = (slice_rows + -(-parts // 16) + 16) * 2.0 ** -23
+    assert bool(((dW.double() - d.t() @ x).abs() <= tol * (d.abs().t() @ x.abs())).all())
+    assert bool(((db.double() - d.sum(0)).abs() <= tol * d.abs().sum(0)).all())
+    again = mx8.linear_wgrad(q, dy)
+    assert torch.equal(dW, again[0]) and torch.equal(db, again[1])
