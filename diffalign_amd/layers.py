@@ -34,6 +34,8 @@ class NodeEdgeBlock(nn.Module):
     `score_cap`, `scope` (improved only; not in the reference): the head's score s becomes score_cap tanh(s / score_cap) where
     score_cap > 0; the softmax runs over 'all' keys (the reference: padded ones too), over the 'nodes' that are real, or over the real
     nodes of the query's own 'side' (product or reactants)."""
+    score_cap, scope = 0.0, 'all'        # (of a module that was pickled whole before it had these)
+
     def __init__(self, dx, de, dy, n_head, improved=False, score_cap=0.0, scope='all', **kwargs):
         super().__init__()
         self.improved = improved

@@ -77,3 +77,24 @@ def test_c_entries_refuse_more_than_a_launch_holds():
     bwd = lambda B, n: lib.da_attn_head_bwd(p, p, p, p, 0, 0, p, 1.0, 0.0, p, p, p, p, 0, p, p, p, p, p, p, p, 1 << 60, B, n, 64, 4, 0)
     for call, B, n in ((fwd, 1 << 24, 1), (fwd, 1 << 23, 3), (bwd, 1 << 23, 1), (bwd, 1 << 21, 100)):
         assert call(B, n) == -1 and b'launch' in lib.da_last_error() and str(B).encode() in lib.da_last_error()
+
+
+def test_a_module_pickled_without_the_attentions_options():
+    """A whole module that torch.save wrote before the block had a cap and a scope: the reference's arithmetic."""
+    import io
+    import torch.nn as nn
+    from diffalign_amd.transformer_model_with_y import GraphTransformerWithY
+    dims = dict(X=16, E=16, y=16)
+    m = GraphTransformerWithY(2, dims, dims, dict(dx=16, de=16, dy=16, n_head=2, dim_ffX=16, dim_ffE=16), dims, nn.ReLU(), nn.ReLU(), improved=True)
+    for layer in m.tf_layers:
+        del layer.self_attn.__dict__['score_cap'], layer.self_attn.__dict__['scope']
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    old = torch.load(f, weights_only=False)
+    assert TF._attn_groups(old, torch.ones(2, 3, dtype=torch.bool), None) is None
+    t, nm, gr, _, _ = inputs(2, 3, 16, 2, 1, False)
+    em = (nm[:, :, None] & nm[:, None, :]).float()[..., None]
+    Y, wV = TF._head_attention_torch(old.tf_layers[1].self_attn, *[x.float() for x in t], em, None)
+    want = O.forward(*t, nm, 2)
+    assert float((Y - want[0]).abs().max()) < 1e-4 and float((wV - want[1]).abs().max()) < 1e-4
