@@ -16,8 +16,8 @@
 // rows, whose Q (dwV, dQ) never move; K_j and V_j are fetched once for the RW rows.  A head's sum runs over df / C neighbouring lanes
 // (DPP).  E1 and E2 are read through a buffer descriptor whose range ends at the rows in hand: a masked pair, a row past the end and a
 // channel past dx get an offset outside it, so the hardware returns the 0 that the formula wants and moves no data.
-// Measured, dx = 256, 8 heads, graphs padded by a quarter on average: B = 16, n = 140 bf16 forward 88 us, backward 136 us (607 MB, 4.5 TB/s) + fold
-// 6.7; B = 16, n = 300 bf16 with 8-bit E1, cap and groups 452 us (2.0 GB, 4.5 TB/s), 526 us (2.5 GB, 4.75 TB/s) + 19; B = 16, n = 140 fp32 158,
+// Measured, dx = 256, 8 heads, graphs padded by a quarter on average: B = 16, n = 140 bf16 forward 88 us, backward 135 us (607 MB, 4.5 TB/s) + fold
+// 6.8; B = 16, n = 300 bf16 with 8-bit E1, cap and groups 449 us (2.0 GB, 4.5 TB/s), 528 us (2.5 GB, 4.75 TB/s) + 19; B = 16, n = 140 fp32 158,
 // 256 + 6.8 us.  A copy of 4 GiB runs at 4.75 TB/s on the same card.
 #include "mfma_util.h"
 #include "mx8_util.h"

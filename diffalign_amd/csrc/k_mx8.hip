@@ -10,7 +10,7 @@
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Quantise / restore.  Streaming: D (s + 1 + 1/32) bytes per row, a dozen integer and float operations per element.  HBM-bound: 313,600 x 256
 // bf16 (243 MB each way) 47 us = 5.2 TB/s to quantise, 34 us to restore right after (the codes are still in the 256 MB cache; non-temporal
-// stores of them cost both: 52 and 39 us).
+// stores of them cost both: 52 and 39 us); fp32 (404 MB) 76 us to quantise = 5.3 TB/s.
 __device__ __forceinline__ void ld8(const float* p, float (&v)[8]) {
   const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
   v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(256) k_mx8_dequant_any(const int8_t* __restric
   }
 }
 
-// dx = dy * scale where the code is not 0 (the forward result was not zero: passed the ReLU and kept by the dropout), else 0
+// dx = dy * scale where the code is not 0 (the forward result was not zero: passed the ReLU and kept by the dropout), else 0.  HBM-bound, 1 + 2 s
+// bytes an element: 313,600 x 128 bf16 (201 MB) 32 us, fp32 (361 MB) 67 us = 5.4 TB/s (a copy of 4 GiB: 4.75; part of dy is still cached).
 template <class T>
 __global__ void __launch_bounds__(256) k_relu_drop_bwd_mx8(const uint2* __restrict__ codes, const T* __restrict__ dy, T* __restrict__ dx, long long octs,
                                                            float scale) {
@@ -119,8 +120,8 @@ __global__ void __launch_bounds__(256) k_relu_drop_bwd_mx8_any(const int8_t* __r
 // toward zero: the whole significand, down to 2^-133, the unit of the subnormal bf16, which the instruction takes as they are), one product
 // each, so nothing of it is rounded away.  Products are exact, sums fp32.
 // A tile's next rows are loaded into registers while the matrix instructions of the present one run (a second LDS buffer in place of the second
-// barrier changes nothing).  313,600 rows: 64 -> 256 bf16 40 us (181 MB, 4.5 TB/s), 256 -> 64 fp32 50 us (163 MB, 3.3 TB/s: three products
-// and 256 conversions a row beside the stream), and 8 us for the fold of 512 partial results.
+// barrier changes nothing).  313,600 rows: 64 -> 256 bf16 41 us (181 MB, 4.5 TB/s), 256 -> 64 fp32 50 us (163 MB, 3.3 TB/s: neither HBM nor the
+// VALU, busy 48 %, is full; a tile's load, stage, products and two barriers follow one another), and 8 us for the fold of 512 partial results.
 // Row pitch in LDS: OUT or IN elements + 64 bytes from 64 features on -- the four rows of a transposing read then start 16 banks apart.
 __host__ __device__ constexpr int tr_pitch(int feats) { return feats * 2 + (feats >= 64 ? 64 : 0); }   // bytes
 
@@ -303,8 +304,12 @@ __global__ void __launch_bounds__(256) k_mx8_wgrad_fold(const float4* __restrict
 }
 
 // Rows of a slice, a multiple of 64.  Up to 131,072 rows 256 slices (one workgroup a CU), beyond that 512: the second workgroup hides the
-// first one's waits, and its partial result costs the fold.  256 / 512 slices, kernel and fold: 64 -> 256 bf16 60,000 rows 18 / 21 us,
-// 313,600 rows 42 / 40 us; 128 -> 64 14 / 18 us, 28 / 25 us.
+// first one's waits, and its partial result costs the fold.  The two cross between 80,000 and 150,000 rows, by shape; 256 / 512 slices, us a call:
+//   rows             60,000     100,000     131,072     150,000     220,000     313,600
+//   64 -> 256 bf16   17.7/20.3  21.5/24.7   28.9/31.4   31.7/31.3   41.7/38.8   53.0/47.7
+//   128 -> 64 bf16   15.0/18.3  17.2/17.1   17.5/17.5   19.7/18.4   24.0/21.5   36.3/27.8
+//   256 -> 64 fp32   21.6/22.5  27.7/26.5   31.7/29.9   36.6/32.3   47.0/42.7   61.9/52.3
+//   64 -> 64 fp32    14.3/15.6  17.1/16.2   19.1/17.2   21.2/18.5   30.2/23.4   41.0/29.8
 static long long wgrad_slice_rows(long long R) {
   const long long G = R <= 131072 ? 256 : 512, per = (R + G - 1) / G;
   return (per + 63) / 64 * 64;

@@ -1,6 +1,7 @@
 // MXINT8 (OCP microscaling): 32 consecutive channels of a row share a power-of-two scale X = 2^(b - 127), one byte b; an element is an
 // int8 q and stands for q / 64 * X.  b is the smallest exponent at which the group's largest magnitude rounds to 127 or less, so
-// every value is within half a step, X / 128, of its element (an amax over 127.5 / 64 * 2^127 has no such b and saturates at 127).
+// every value is within half a step, X / 128, of its element (an amax over 127.5 / 64 * 2^127 has no such b and saturates at 127; KEEP lifts
+// an element below half a step to a whole one).
 // b as written is in [MX8_B_MIN, 254]: X >= 2^-100 keeps every element a normal bf16 / fp32 (smaller values round to zero at that step); any
 // byte is read.
 // A group with an infinity or NaN gets b = 255 and stands for NaN throughout.  An element has 7 significant bits: exact in bf16.

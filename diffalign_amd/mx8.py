@@ -2,9 +2,11 @@
 
 Format: MXINT8 of the OCP microscaling specification.  32 consecutive channels of a row share a power-of-two scale 2^(b - 127), held as one
 byte b; an element is an int8 q and stands for q / 64 * 2^(b - 127).  The scale is the smallest at which the group's largest magnitude
-still rounds to 127, so a restored value is within half a step, 2^(b - 127) / 128, of the original (at most 1/127 of the group's
-largest magnitude); restored values are exact in bfloat16.  Scales go down to 2^-100: smaller values round to zero at that step.  A
-group that holds an infinity or NaN is restored as NaN.  D channels take D + ceil(D / 32) bytes.
+still rounds to 127, so a restored value is within half a step, 2^(b - 127) / 128, of the original: at most 1/127 of the group's
+largest magnitude.  With keep_nonzero what would round to zero gets a whole step instead, up to 1/63.5 of that magnitude and, after a
+ReLU, always upward.  Restored values are exact in bfloat16.  Written scales go down to 2^-100, so a group whose largest magnitude is below
+about 2^-100 is held in steps of 2^-106; read, any scale byte stands for its power of two, 255 for NaN.  A group that holds an infinity or
+NaN is restored as NaN.  D channels take D + ceil(D / 32) bytes.
 
 The reference keeps every activation at full width for `loss.backward()` (training/helpers.py:139-142); the callers here are the training
 forward's per-pair Linears and the per-head attention core (train_forward.py, `train_checkpoint = 'mx8'`).  The functions here are what

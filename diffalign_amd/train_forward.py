@@ -273,8 +273,8 @@ PRECISION = _os.environ.get('DA_TRAIN_PRECISION', 'fp32')
 # 'none' (default: the backward gets every activation as the forward had it) or 'mx8': the inputs of the per-pair Linears of the layers, and in the
 # improved block the attention's E1, are held in 8 bits between the two passes (mx8.py).  The gradients of those weights, and dQ and dK of the
 # per-head attention, see the rounded values; the plain block's forward does not change.  Goes with the fused residual blocks, which the
-# improved block takes only here (its dropout masks are then the hash's, and in mixed precision its per-pair tensors bf16 as well).  Set per
-# module (`module.train_checkpoint = 'mx8'`) or process-wide here / by DA_TRAIN_CHECKPOINT.
+# improved block takes only here (its dropout masks are then the hash's, and in mixed precision its per-pair tensors bf16 as well); a layer whose
+# widths have none is refused.  Set per module (`module.train_checkpoint = 'mx8'`) or process-wide here / by DA_TRAIN_CHECKPOINT.
 CHECKPOINT = _os.environ.get('DA_TRAIN_CHECKPOINT', 'none')
 
 
