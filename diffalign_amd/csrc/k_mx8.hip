@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256) k_relu_drop_bwd_mx8_any(const int8_t* __r
 // each, so nothing of it is rounded away.  Products are exact, sums fp32.
 // A tile's next rows are loaded into registers while the matrix instructions of the present one run (a second LDS buffer in place of the second
 // barrier changes nothing).  313,600 rows: 64 -> 256 bf16 41 us (181 MB, 4.5 TB/s), 256 -> 64 fp32 50 us (163 MB, 3.3 TB/s: neither HBM nor the
-// VALU, busy 48 %, is full; a tile's load, stage, products and two barriers follow one another), and 8 us for the fold of 512 partial results.
+// VALU, busy 52 %, is full; a tile's load, stage, products and two barriers follow one another), and 8 us for the fold of 512 partial results.
 // Row pitch in LDS: OUT or IN elements + 64 bytes from 64 features on -- the four rows of a transposing read then start 16 banks apart.
 __host__ __device__ constexpr int tr_pitch(int feats) { return feats * 2 + (feats >= 64 ? 64 : 0); }   // bytes
 
